@@ -147,7 +147,8 @@ def prepare(case: dict, seed: int) -> dict:
     if own:
         from cross_dsl_kernels_b200.kv8 import PagedKV8Cache
 
-        st["cache"] = PagedKV8Cache(st["k_cache"], st["v_cache"], st["k_scale"], st["v_scale"], st["k_mean"], kv_layout=layout)
+        v_codes = torch.empty_like(k_codes) if kind == "select" else v_codes  # the tensors of a cache are apart
+        st["cache"] = PagedKV8Cache(st["k_cache"], v_codes, st["k_scale"], st["v_scale"], st["k_mean"], kv_layout=layout)
     return st
 
 
