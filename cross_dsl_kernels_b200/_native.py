@@ -16,6 +16,7 @@ import warnings
 LIB_PATH = pathlib.Path(__file__).resolve().parent / "libxdk_b200.so"
 
 XDK_F32, XDK_BF16, XDK_F16 = 0, 1, 2
+XDK_KV8_INT8, XDK_KV8_E4M3 = 0, 1  # code types of the 8-bit K/V cache
 XDK_STRICT_FP32, XDK_DEPENDENT_LAUNCH = 1, 2  # flags of the *_v2 entry points
 
 _p = ctypes.c_void_p
@@ -48,6 +49,12 @@ SIGNATURES = {
     "xdk_paged_decode_attention_scratch_bytes": (ctypes.c_size_t, [_i64] * 5 + [_int]),
     "xdk_paged_decode_attention_ws": (_int, [_p] * 7 + [_i64] * 6 + [_int, ctypes.c_float, _i64, _int, _p, ctypes.c_size_t, _uint, _p]),
     "xdk_swiglu_peer": (_int, [_p, _p, _i64, _i64, _i64, _int, _uint, _p]),
+    "xdk_kv8_append_scratch_bytes": (ctypes.c_size_t, [_i64]),
+    "xdk_kv8_append": (_int, [_p] * 14 + [_i64] * 11 + [_int] * 4 + [_p, ctypes.c_size_t, _uint, _p]),
+    "xdk_kv8_decode_attention_scratch_bytes": (ctypes.c_size_t, [_i64] * 5),
+    "xdk_kv8_decode_attention": (_int, [_p] * 9 + [_i64] * 6 + [_int, ctypes.c_float, _i64, _int, _int, _p, ctypes.c_size_t, _uint, _p]),
+    "xdk_kv8_select_pages": (_int, [_p] * 7 + [_i64] * 7 + [_int, _uint, _p]),
+    "xdk_kv8_sparse_attention": (_int, [_p] * 10 + [_i64] * 7 + [_int, ctypes.c_float, _int, _int, _uint, _p]),
     "xdk_quantize_int4": (_int, [_p, _int, _i64, _i64, _int, _p, _p, _p, _p]),
     "xdk_peer_fault_flags": (ctypes.c_uint, []),
     "xdk_peer_alloc": (_int, [ctypes.c_size_t, _p]),

@@ -1,4 +1,4 @@
-// The eager calls of ops.py and w4a16.py in native code: check the tensors, allocate the outputs, launch.
+// The eager calls of ops.py, w4a16.py and kv8.py in native code: check the tensors, allocate the outputs, launch.
 //
 // A decode step called eagerly is bound by the host: the checks and the ctypes call of one op took 17 - 75 us of Python,
 // several times the kernel.  Here they take 5 (a BF16 norm of 16 x 4096: 18.7 -> 5.9 us a call; an append of few tokens:
@@ -321,13 +321,170 @@ PyObject* swiglu(PyObject*, PyObject* const* arg, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---- the 8-bit paged cache (kv8.py) --------------------------------------------------------------------------------------
+// What its four ops share: q, the cache as (k, v, k_scale, v_scale, k_mean or None, kv_layout), and the three index tensors.  The
+// tensors of a cache were checked against one another when it was made.
+struct Kv8Call {
+  const at::Tensor *q, *k, *v, *ks, *vs, *mean, *pos, *table, *seq;
+  int hnd, code, codes;
+  int64_t tokens, hq, hkv, dim, page, width;
+  bool read(PyObject* const* cache, PyObject* q_arg, PyObject* const* index) {
+    q = tensor_of(q_arg), k = tensor_of(cache[0]), v = tensor_of(cache[1]), ks = tensor_of(cache[2]), vs = tensor_of(cache[3]);
+    mean = cache[4] == Py_None ? nullptr : tensor_of(cache[4]);
+    pos = tensor_of(index[0]), table = tensor_of(index[1]), seq = tensor_of(index[2]);
+    if (!q || !k || !v || !ks || !vs || !pos || !table || !seq || (!mean && cache[4] != Py_None)) return false;
+    hnd = layout_of(cache[5]), code = dtype_code(q->scalar_type());
+    codes = k->scalar_type() == at::kChar ? XDK_KV8_INT8 : XDK_KV8_E4M3;
+    if (hnd < 0 || code < 0 || q->dim() != 3 || q->numel() == 0 || q->requires_grad() || k->device() != q->device() || !sm100(*q)) return false;
+    tokens = q->size(0), hq = q->size(1), dim = q->size(2), hkv = k->size(hnd ? 1 : 2), page = k->size(hnd ? 2 : 1);
+    if (k->size(3) != dim || hq % hkv != 0) return false;
+    for (const at::Tensor* t : {pos, table, seq})
+      if (t->device() != q->device() || t->scalar_type() != at::kLong || !t->is_contiguous()) return false;
+    if (pos->dim() != 1 || seq->dim() != 1 || table->dim() != 2 || pos->size(0) != tokens || seq->size(0) != tokens || table->numel() == 0)
+      return false;
+    width = table->size(1);
+    return true;
+  }
+  bool reads() const { return q->is_contiguous() && hq / hkv <= 8; }
+  xdk_peer_out to(const at::Tensor& out) const {
+    xdk_peer_out dst = {};
+    dst.ptr[0] = out.data_ptr(), dst.world = 1, dst.ld = hq * dim, dst.col0 = 0;
+    return dst;
+  }
+};
+bool scale_of(PyObject* o, int64_t dim, double& scale) {
+  if (o != Py_None && !PyFloat_CheckExact(o)) return false;
+  scale = o == Py_None ? std::pow(static_cast<double>(dim), -0.5) : PyFloat_AS_DOUBLE(o);
+  return std::isfinite(scale);
+}
+
+// (q, k, v, cos, sin, positions, page_table, sequence_ids, <cache: 6>, rope_dim, interleaved, dependent_launch)
+PyObject* kv8_append(PyObject*, PyObject* const* arg, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  NEED(n == 17);
+  Kv8Call c;
+  int64_t rope;
+  bool interleaved, dep;
+  NEED(int_of(arg[14], rope) && flag_of(arg[15], interleaved) && flag_of(arg[16], dep) && c.read(arg + 8, arg[0], arg + 5));
+  const at::Tensor *k = tensor_of(arg[1]), *v = tensor_of(arg[2]), *cos = tensor_of(arg[3]), *sin = tensor_of(arg[4]);
+  NEED(k && v && cos && sin);
+  for (const at::Tensor* t : {k, v, cos, sin})
+    NEED(t->device() == c.q->device() && !t->requires_grad() && t->scalar_type() == (t == k || t == v ? c.q->scalar_type() : at::kFloat));
+  NEED(k->dim() == 3 && k->size(0) == c.tokens && k->size(1) == c.hkv && k->size(2) == c.dim && v->sizes() == k->sizes());
+  for (const at::Tensor* t : {c.q, k, v})
+    NEED(t->is_contiguous() || (t->stride(2) == 1 && t->stride(1) == t->size(2) && t->stride(0) >= t->size(1) * t->size(2)));
+  NEED(rope > 0 && rope % 2 == 0 && rope <= c.dim && cos->dim() == 2 && cos->is_contiguous() && sin->is_contiguous());
+  NEED(cos->size(0) > 0 && cos->size(1) >= rope / 2 && sin->sizes() == cos->sizes());
+  for (const at::Tensor* t : {c.q, k, v, cos, sin, c.pos, c.table, c.seq})
+    for (const at::Tensor* own : {c.k, c.v, c.ks, c.vs, c.mean}) NEED(!own || !overlaps(*own, *t));
+  at::Tensor out;
+  int st;
+  {
+    Unlocked unlocked;
+    c10::cuda::CUDAGuard guard(c.q->device());
+    out = at::empty(c.q->sizes(), c.q->options());
+    const size_t need = xdk_kv8_append_scratch_bytes(c.tokens);
+    at::Tensor scratch;
+    if (need) scratch = at::empty({static_cast<int64_t>(need)}, c.q->options().dtype(at::kByte));
+    const bool many = c.tokens > 1;
+    st = xdk_kv8_append(c.q->data_ptr(), k->data_ptr(), v->data_ptr(), cos->const_data_ptr<float>(), sin->const_data_ptr<float>(),
+                        c.pos->const_data_ptr<int64_t>(), c.table->const_data_ptr<int64_t>(), c.seq->const_data_ptr<int64_t>(), out.data_ptr(),
+                        c.k->data_ptr(), c.v->data_ptr(), c.ks->mutable_data_ptr<float>(), c.vs->mutable_data_ptr<float>(),
+                        c.mean ? c.mean->mutable_data_ptr<int8_t>() : nullptr, c.tokens, c.hq, c.hkv, c.dim, cos->size(1), c.width, c.page,
+                        rope, many ? c.q->stride(0) : c.hq * c.dim, many ? k->stride(0) : c.hkv * c.dim, many ? v->stride(0) : c.hkv * c.dim,
+                        interleaved, c.hnd, c.code, c.codes, need ? scratch.data_ptr() : nullptr, need, launch_flags(dep), stream_of(*c.q));
+  }
+  return finish(st, "xdk_kv8_append", THPVariable_Wrap(std::move(out)));
+  END_HANDLE_TH_ERRORS
+}
+
+// (q, <cache: 6>, positions, page_table, sequence_ids, scale or None, context_hint, dependent_launch)
+PyObject* kv8_attention(PyObject*, PyObject* const* arg, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  NEED(n == 13);
+  Kv8Call c;
+  int64_t hint;
+  double scale;
+  bool dep;
+  NEED(int_of(arg[11], hint) && flag_of(arg[12], dep) && c.read(arg + 1, arg[0], arg + 7) && c.reads() && scale_of(arg[10], c.dim, scale));
+  if (hint <= 0 && __builtin_mul_overflow(c.width, c.page, &hint)) NOT_MINE;  // no bound: that of a page table row
+  at::Tensor out;
+  int st;
+  {
+    Unlocked unlocked;
+    c10::cuda::CUDAGuard guard(c.q->device());
+    out = at::empty_like(*c.q);
+    const size_t need = xdk_kv8_decode_attention_scratch_bytes(c.tokens, c.hq, c.hkv, c.dim, hint);
+    at::Tensor scratch;
+    if (need) scratch = at::empty({static_cast<int64_t>(need)}, c.q->options().dtype(at::kByte));
+    const xdk_peer_out dst = c.to(out);
+    st = xdk_kv8_decode_attention(c.q->data_ptr(), c.k->data_ptr(), c.v->data_ptr(), c.ks->const_data_ptr<float>(), c.vs->const_data_ptr<float>(),
+                                  c.pos->const_data_ptr<int64_t>(), c.table->const_data_ptr<int64_t>(), c.seq->const_data_ptr<int64_t>(), &dst,
+                                  c.tokens, c.hq, c.hkv, c.dim, c.width, c.page, c.hnd, static_cast<float>(scale), hint, c.code, c.codes,
+                                  need ? scratch.data_ptr() : nullptr, need, launch_flags(dep), stream_of(*c.q));
+  }
+  return finish(st, "xdk_kv8_decode_attention", THPVariable_Wrap(std::move(out)));
+  END_HANDLE_TH_ERRORS
+}
+
+// (q, <cache: 6>, positions, page_table, sequence_ids, top_pages, dependent_launch)
+PyObject* kv8_select(PyObject*, PyObject* const* arg, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  NEED(n == 12);
+  Kv8Call c;
+  int64_t top;
+  bool dep;
+  NEED(int_of(arg[10], top) && flag_of(arg[11], dep) && c.read(arg + 1, arg[0], arg + 7) && c.reads() && c.mean);
+  NEED(top > 0 && top <= std::numeric_limits<int32_t>::max() && c.width <= 51200);
+  at::Tensor pages;
+  int st;
+  {
+    Unlocked unlocked;
+    c10::cuda::CUDAGuard guard(c.q->device());
+    pages = at::empty({c.tokens, c.hkv, top}, c.q->options().dtype(at::kInt));
+    st = xdk_kv8_select_pages(c.q->data_ptr(), c.mean->const_data_ptr<int8_t>(), c.ks->const_data_ptr<float>(), c.pos->const_data_ptr<int64_t>(),
+                              c.table->const_data_ptr<int64_t>(), c.seq->const_data_ptr<int64_t>(), pages.mutable_data_ptr<int32_t>(), c.tokens,
+                              c.hq, c.hkv, c.dim, c.width, c.page, top, c.code, launch_flags(dep), stream_of(*c.q));
+  }
+  return finish(st, "xdk_kv8_select_pages", THPVariable_Wrap(std::move(pages)));
+  END_HANDLE_TH_ERRORS
+}
+
+// (q, <cache: 6>, pages, positions, page_table, sequence_ids, scale or None, dependent_launch)
+PyObject* kv8_sparse(PyObject*, PyObject* const* arg, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  NEED(n == 13);
+  Kv8Call c;
+  double scale;
+  bool dep;
+  NEED(flag_of(arg[12], dep) && c.read(arg + 1, arg[0], arg + 8) && c.reads() && scale_of(arg[11], c.dim, scale));
+  const at::Tensor* pages = tensor_of(arg[7]);
+  NEED(pages && pages->device() == c.q->device() && pages->scalar_type() == at::kInt && pages->is_contiguous() && pages->dim() == 3);
+  NEED(pages->size(0) == c.tokens && pages->size(1) == c.hkv && pages->size(2) > 0 && pages->size(2) <= std::numeric_limits<int32_t>::max() / 1024);
+  at::Tensor out;
+  int st;
+  {
+    Unlocked unlocked;
+    c10::cuda::CUDAGuard guard(c.q->device());
+    out = at::empty_like(*c.q);
+    const xdk_peer_out dst = c.to(out);
+    st = xdk_kv8_sparse_attention(c.q->data_ptr(), c.k->data_ptr(), c.v->data_ptr(), c.ks->const_data_ptr<float>(), c.vs->const_data_ptr<float>(),
+                                  pages->const_data_ptr<int32_t>(), c.pos->const_data_ptr<int64_t>(), c.table->const_data_ptr<int64_t>(),
+                                  c.seq->const_data_ptr<int64_t>(), &dst, c.tokens, c.hq, c.hkv, c.dim, c.width, c.page, pages->size(2), c.hnd,
+                                  static_cast<float>(scale), c.code, c.codes, launch_flags(dep), stream_of(*c.q));
+  }
+  return finish(st, "xdk_kv8_sparse_attention", THPVariable_Wrap(std::move(out)));
+  END_HANDLE_TH_ERRORS
+}
+
 PyObject* set_check(PyObject*, PyObject* fn) {
   Py_XSETREF(g_check, Py_NewRef(fn));
   Py_RETURN_NONE;
 }
 
 #define FAST(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
-PyMethodDef g_methods[] = {FAST(rmsnorm), FAST(linear), FAST(w4a16), FAST(append), FAST(attention), FAST(swiglu),
+PyMethodDef g_methods[] = {FAST(rmsnorm), FAST(linear), FAST(w4a16), FAST(append), FAST(attention), FAST(swiglu), FAST(kv8_append),
+                           FAST(kv8_attention), FAST(kv8_select), FAST(kv8_sparse),
                            {"set_check", set_check, METH_O, nullptr}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -1,0 +1,239 @@
+// Which pages of an 8-bit paged cache (kv8.cuh) a query reads: the ones whose mean key scores best.
+//
+//   codes of q, per head: qc = rint(q / unit), unit = max |q| * (1 / 127)         (q = qc * unit to half a unit)
+//   score of a page in front of the token's last one: max over the heads of a group of (unit * (qc . mean)) * scale of the block
+//   chosen: the top_pages - 1 best of them (the lowest page first among equals), and the last page always
+// The dot products are sums of whole numbers below 2^24 and every other step is one correctly rounded FP32 operation, so the choice is
+// the same whatever computes it.  One choice per token and KV head: the query heads that share it read its pages together.
+//
+// One CTA per (token, KV head).  Scores: mma.m16n8k32 on bytes, 16 pages as rows, the heads of the group as columns; a thread
+// loads a quarter of two pages' means with 16-byte loads, and the codes of q stand in registers in the same order of dims.  The scores
+// stay in shared memory as sortable integers; four passes over their bytes find the value of the last one chosen, a fifth writes
+// the pages in order.  Bound: short contexts by the chain of launches and barriers, long ones by the reads of the means.
+#include <math.h>
+
+#include "kv8.cuh"
+
+namespace xdk {
+namespace {
+
+constexpr int kSelThreads = 512, kSelWarps = kSelThreads / 32;
+constexpr int64_t kMaxCandidates = 51200;  // keys in shared memory
+
+struct SelectArgs {
+  const void* q;
+  const int8_t* k_mean;
+  const float* k_scale;
+  const int64_t *positions, *page_table, *sequence_ids;
+  int32_t* pages;
+  int64_t max_pages;
+  int q_heads, kv_heads, page_size, top_pages;
+};
+
+__device__ __forceinline__ void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// Larger key: larger score; one that is not a number (a block with such a value) before all others.
+__device__ __forceinline__ uint32_t key_of(float score) {
+  if (score != score) return 0xffffffffu;
+  const uint32_t b = __float_as_uint(score + 0.0f);  // -0 and 0 are equals
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kSelThreads)
+kv8_select_kernel(const __grid_constant__ SelectArgs a) {
+  constexpr int kWords = D / 16;  // of four dims, per thread and page
+  extern __shared__ uint32_t keys[];
+  __shared__ __align__(16) uint32_t codes[8][D / 4];
+  __shared__ float unit[8];
+  __shared__ unsigned bins[256];
+  __shared__ unsigned warp_sum[8], chosen[2];
+  __shared__ int warp_above[kSelWarps], warp_equal[kSelWarps];
+
+  pdl_launch_dependents();
+  pdl_wait();
+  const int token = blockIdx.y, kvh = blockIdx.x;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int group = a.q_heads / a.kv_heads;
+  int32_t* out = a.pages + (static_cast<int64_t>(token) * a.kv_heads + kvh) * a.top_pages;
+  const int64_t pos = a.positions[token];
+  if (pos < 0) {
+    for (int i = tid; i < a.top_pages; i += kSelThreads) out[i] = -1;
+    return;
+  }
+  const int64_t at_page = pos / a.page_size;
+  const int last = static_cast<int>(at_page < a.max_pages ? at_page : a.max_pages - 1);
+  const int want = a.top_pages - 1;  // of the pages in front of the last one
+  if (last <= want) {
+    for (int i = tid; i < a.top_pages; i += kSelThreads) out[i] = i <= last ? i : -1;
+    return;
+  }
+  const int64_t* table = a.page_table + a.sequence_ids[token] * a.max_pages;
+
+  if (warp < 8) {  // codes of head `warp` of the group, zeros for a head that is none
+    constexpr int N = D / 32;
+    float x[N], top = 0.0f;
+    const T* q = static_cast<const T*>(a.q) + (static_cast<int64_t>(token) * a.q_heads + kvh * group + warp) * D + lane * N;
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      x[e] = warp < group ? Elem<T>::to_f32(q[e]) : 0.0f;
+      top = fmaxf(top, fabsf(x[e]));
+    }
+#pragma unroll
+    for (int sh = 16; sh > 0; sh >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, sh));
+    const float u = __fmul_rn(top, 1.0f / 127.0f);
+    if (lane == 0) unit[warp] = u;
+    int8_t* to = reinterpret_cast<int8_t*>(codes[warp]) + lane * N;
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const float c = u > 0.0f ? fminf(fmaxf(rintf(__fdiv_rn(x[e], u)), -127.0f), 127.0f) : 0.0f;
+      to[e] = static_cast<int8_t>(static_cast<int>(c));
+    }
+  }
+  __syncthreads();
+
+  // ---- scores
+  const int row = lane >> 2, quad = lane & 3;
+  uint32_t b[kWords];  // head `row`, dims quad * D / 4 ..
+#pragma unroll
+  for (int w = 0; w < kWords; ++w) b[w] = codes[row][quad * kWords + w];
+  const float unit0 = unit[2 * quad], unit1 = unit[2 * quad + 1];
+  const bool live0 = 2 * quad < group, live1 = 2 * quad + 1 < group;
+  for (int base = warp * 16; base < last; base += kSelWarps * 16) {
+    const int p0 = base + row, p1 = p0 + 8;
+    const int64_t block0 = (p0 < last ? table[p0] : table[base]) * a.kv_heads + kvh, block1 = (p1 < last ? table[p1] : table[base]) * a.kv_heads + kvh;
+    uint32_t m0[kWords], m1[kWords];
+#pragma unroll
+    for (int w = 0; w < kWords; w += 4) {
+      const U4 v0 = ld_ordered_stream16(a.k_mean + block0 * D + quad * (D / 4) + w * 4);
+      const U4 v1 = ld_ordered_stream16(a.k_mean + block1 * D + quad * (D / 4) + w * 4);
+      m0[w] = v0.x, m0[w + 1] = v0.y, m0[w + 2] = v0.z, m0[w + 3] = v0.w;
+      m1[w] = v1.x, m1[w + 1] = v1.y, m1[w + 2] = v1.z, m1[w + 3] = v1.w;
+    }
+    const float scale0 = a.k_scale[block0], scale1 = a.k_scale[block1];
+    int dot[4] = {};
+#pragma unroll
+    for (int w = 0; w < kWords; w += 2) mma_s8(dot, m0[w], m1[w], m0[w + 1], m1[w + 1], b[w], b[w + 1]);
+    float s[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const float x = live0 ? __fmul_rn(static_cast<float>(dot[2 * e]), unit0) : -INFINITY;
+      const float y = live1 ? __fmul_rn(static_cast<float>(dot[2 * e + 1]), unit1) : -INFINITY;
+      s[e] = fmaxf(x, y);
+#pragma unroll
+      for (int sh = 1; sh < 4; sh <<= 1) s[e] = fmaxf(s[e], __shfl_xor_sync(0xffffffffu, s[e], sh));
+    }
+    if (quad == 0 && p0 < last) keys[p0] = key_of(__fmul_rn(s[0], scale0));
+    if (quad == 1 && p1 < last) keys[p1] = key_of(__fmul_rn(s[1], scale1));
+  }
+
+  // ---- the key of the last one chosen, byte by byte from the top; `left`: how many of the keys that agree so far are wanted
+  uint32_t prefix = 0;
+  unsigned left = static_cast<unsigned>(want);
+  if (want > 0) {
+    for (int shift = 24; shift >= 0; shift -= 8) {
+      if (tid < 256) bins[tid] = 0;
+      __syncthreads();
+      const uint32_t mask = shift == 24 ? 0u : 0xffffffffu << (shift + 8);
+      for (int i = tid; i < last; i += kSelThreads)
+        if ((keys[i] & mask) == prefix) atomicAdd(&bins[keys[i] >> shift & 255u], 1u);
+      __syncthreads();
+      unsigned mine = 0, upto = 0;
+      if (tid < 256) {  // thread t: bin 255 - t; keys in it and in those above
+        mine = upto = bins[255 - tid];
+#pragma unroll
+        for (int sh = 1; sh < 32; sh <<= 1) {
+          const unsigned v = __shfl_up_sync(0xffffffffu, upto, sh);
+          if (lane >= sh) upto += v;
+        }
+        if (lane == 31) warp_sum[warp] = upto;
+      }
+      __syncthreads();
+      if (tid < 256) {
+        for (int w = 0; w < warp; ++w) upto += warp_sum[w];
+        if (upto - mine < left && left <= upto) chosen[0] = 255u - tid, chosen[1] = left - (upto - mine);
+      }
+      __syncthreads();
+      prefix |= chosen[0] << shift, left = chosen[1];
+    }
+  } else {
+    prefix = 0xffffffffu, left = 0;
+    __syncthreads();
+  }
+
+  // ---- pages whose key is above, and the first `left` of the equals, in order
+  int above = 0, equal = 0;  // in front of this round of pages
+  for (int base = 0; base < last; base += kSelThreads) {
+    const int p = base + tid;
+    const uint32_t key = p < last ? keys[p] : 0u;
+    const unsigned is_above = __ballot_sync(0xffffffffu, p < last && want > 0 && key > prefix);
+    const unsigned is_equal = __ballot_sync(0xffffffffu, p < last && want > 0 && key == prefix);
+    if (lane == 0) warp_above[warp] = __popc(is_above), warp_equal[warp] = __popc(is_equal);
+    __syncthreads();
+    const unsigned before = (1u << lane) - 1u;
+    int my_above = above + __popc(is_above & before), my_equal = equal + __popc(is_equal & before);
+    for (int w = 0; w < kSelWarps; ++w) {
+      if (w < warp) my_above += warp_above[w], my_equal += warp_equal[w];
+      above += warp_above[w], equal += warp_equal[w];
+    }
+    const int limit = static_cast<int>(left);
+    const bool taken = (is_above >> lane & 1u) || ((is_equal >> lane & 1u) && my_equal < limit);
+    if (taken) out[my_above + (my_equal < limit ? my_equal : limit)] = p;
+    __syncthreads();
+  }
+  if (tid == 0) out[want] = last;
+}
+
+template <typename T>
+int dispatch_select(int64_t d, const SelectArgs& a, dim3 grid, size_t smem, cudaStream_t s) {
+  auto run = [&](auto kernel) {
+    if (smem > 40 * 1024) {  // with what it has statically, beyond what a launch gets unasked
+      const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+      if (err != cudaSuccess) return note_launch(err);
+    }
+    return launch_dependent(kernel, grid, dim3(kSelThreads), smem, s, a);
+  };
+  switch (d) {
+    case 64: return run(kv8_select_kernel<T, 64>);
+    case 128: return run(kv8_select_kernel<T, 128>);
+    case 256: return run(kv8_select_kernel<T, 256>);
+    default: return XDK_ERR_LIMIT;
+  }
+}
+
+}  // namespace
+}  // namespace xdk
+
+extern "C" int xdk_kv8_select_pages(const void* q, const int8_t* k_mean, const float* k_scale, const int64_t* positions,
+                                    const int64_t* page_table, const int64_t* sequence_ids, int32_t* pages, int64_t tokens, int64_t q_heads,
+                                    int64_t kv_heads, int64_t head_dim, int64_t max_pages_per_seq, int64_t page_size, int64_t top_pages,
+                                    int dtype, unsigned flags, void* stream) {
+  using namespace xdk;
+  if (flags & ~XDK_DEPENDENT_LAUNCH) return XDK_ERR_ARG;
+  CallFlagsScope scope(flags);
+  if (!q || !k_mean || !k_scale || !positions || !page_table || !sequence_ids || !pages) return XDK_ERR_ARG;
+  if (tokens < 1 || q_heads < 1 || kv_heads < 1 || head_dim < 1 || page_size < 1 || max_pages_per_seq < 1 || top_pages < 1) return XDK_ERR_ARG;
+  if (q_heads % kv_heads != 0 || !aligned16(k_mean)) return XDK_ERR_ARG;
+  if (dtype != XDK_F32 && dtype != XDK_BF16 && dtype != XDK_F16) return XDK_ERR_ARG;
+  if (!kv8_head_dim(head_dim) || q_heads / kv_heads > 8 || tokens > 65535 || top_pages > 2147483647LL || max_pages_per_seq > kMaxCandidates)
+    return XDK_ERR_LIMIT;
+  if (int st = kv8_limits(tokens, kv_heads, max_pages_per_seq, page_size)) return st;
+  if (int st = require_sm100()) return st;
+  SelectArgs a;
+  a.q = q, a.k_mean = k_mean, a.k_scale = k_scale, a.positions = positions, a.page_table = page_table, a.sequence_ids = sequence_ids;
+  a.pages = pages, a.max_pages = max_pages_per_seq;
+  a.q_heads = static_cast<int>(q_heads), a.kv_heads = static_cast<int>(kv_heads), a.page_size = static_cast<int>(page_size);
+  a.top_pages = static_cast<int>(top_pages);
+  const dim3 grid(static_cast<unsigned>(kv_heads), static_cast<unsigned>(tokens));
+  const size_t smem = static_cast<size_t>(max_pages_per_seq) * 4;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  switch (dtype) {
+    case XDK_F32: return dispatch_select<float>(head_dim, a, grid, smem, s);
+    case XDK_BF16: return dispatch_select<__nv_bfloat16>(head_dim, a, grid, smem, s);
+    case XDK_F16: return dispatch_select<__half>(head_dim, a, grid, smem, s);
+    default: return XDK_ERR_ARG;
+  }
+}

@@ -304,6 +304,57 @@ XDK_API int xdk_swiglu_peer(const void* upgate, const xdk_peer_out* out_dst, int
 
 
 /*
+ * The paged K/V cache in 8 bits (no counterpart in the reference): half the bytes of a 16-bit one.  Codes of one byte, int8 or
+ * e4m3, in the two cache layouts of xdk_rope_kv_append, and per block -- a page of one KV head -- an FP32 scale for K and one for V,
+ * [pages, kv_heads]: a value is code * scale.  k_mean, int8 [pages, kv_heads, head_dim], holds the mean key of each block, for
+ * the selection of pages.  head_dim in {64, 128, 256}, page_size <= 1024; caches, k_mean, scratch 16-byte aligned.
+ *
+ * xdk_kv8_append: the rotation and the append of xdk_rope_kv_append, in any order of tokens and any number of them for a page.  For each
+ *   block, with W its rows that the call writes, top = 127 (int8) or 448 (e4m3):
+ *     before = 0 if row 0 is in W, else its scale; scale = max(before, max |x| of W * (1 / top))
+ *     rows in W: code = round(x / scale), half to even (two tokens for one slot: the one with the larger index); the other rows, if row 0
+ *     is not in W and the scale grew: code = round(code * (before / scale)).
+ *     If the last row is in W, the mean of the block's codes as int8, in units of scale, or of scale * 448 / 127 for e4m3.
+ *   So a page begins anew when its first position is written.  A scale is NaN, and the block reads as NaN, from when it is given a value
+ *   that is not finite until then.  positions[t] < 0 (padding): nothing is written, q_out of the token is 0.  q, k, v are strided as there,
+ *   q_out is contiguous; k_mean may be NULL (no means).  scratch: xdk_kv8_append_scratch_bytes(tokens) bytes (0 for
+ *   small batches), content undefined, not shared by calls that may overlap on the GPU; one memset and two launches then, one launch else.
+ * xdk_kv8_decode_attention: xdk_paged_decode_attention_ws for this cache: any q_heads / kv_heads up to 8; softmax and sums in FP32; a context
+ *   of no positions (positions[t] < 0) gives 0.
+ * xdk_kv8_select_pages: per token and KV head the last page of the context and the top_pages - 1 others with the best scores,
+ *   score = max over the heads of the group of (unit * (qc . k_mean)) * k_scale, qc = round(q / unit), unit = max |q| * (1 / 127), the
+ *   lowest page first among equals.  pages: int32 [tokens, kv_heads, top_pages], logical pages, ascending, -1 behind the last one; all -1 for a
+ *   position < 0.  k_mean has to hold the means of all pages in front of the last one (the append writes them as blocks fill up).
+ *   q_heads / kv_heads <= 8; at most 51200 pages per sequence (XDK_ERR_LIMIT).
+ * xdk_kv8_sparse_attention: the attention over the positions of the listed pages, [tokens, kv_heads, n_pages], ascending; an entry that is
+ *   negative, not above the one before, or behind the context adds nothing.  One launch, no scratch.
+ */
+typedef enum xdk_kv8_codes { XDK_KV8_INT8 = 0, XDK_KV8_E4M3 = 1 } xdk_kv8_codes;
+XDK_API size_t xdk_kv8_append_scratch_bytes(int64_t tokens);
+XDK_API int xdk_kv8_append(const void* q, const void* k, const void* v, const float* cos, const float* sin, const int64_t* positions,
+                   const int64_t* page_table, const int64_t* sequence_ids, void* q_out, void* k_cache, void* v_cache,
+                   float* k_scale, float* v_scale, int8_t* k_mean, int64_t tokens, int64_t q_heads, int64_t kv_heads,
+                   int64_t head_dim, int64_t cos_width, int64_t max_pages_per_seq, int64_t page_size, int64_t rope_dim,
+                   int64_t q_token_stride, int64_t k_token_stride, int64_t v_token_stride, int interleaved, int cache_is_hnd,
+                   int dtype, int codes, void* scratch, size_t scratch_bytes, unsigned flags, void* stream);
+XDK_API size_t xdk_kv8_decode_attention_scratch_bytes(int64_t tokens, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
+                                              int64_t context_hint);
+XDK_API int xdk_kv8_decode_attention(const void* q, const void* k_cache, const void* v_cache, const float* k_scale, const float* v_scale,
+                             const int64_t* positions, const int64_t* page_table, const int64_t* sequence_ids,
+                             const xdk_peer_out* out_dst, int64_t tokens, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
+                             int64_t max_pages_per_seq, int64_t page_size, int cache_is_hnd, float scale, int64_t context_hint,
+                             int dtype, int codes, void* scratch, size_t scratch_bytes, unsigned flags, void* stream);
+XDK_API int xdk_kv8_select_pages(const void* q, const int8_t* k_mean, const float* k_scale, const int64_t* positions,
+                         const int64_t* page_table, const int64_t* sequence_ids, int32_t* pages, int64_t tokens, int64_t q_heads,
+                         int64_t kv_heads, int64_t head_dim, int64_t max_pages_per_seq, int64_t page_size, int64_t top_pages,
+                         int dtype, unsigned flags, void* stream);
+XDK_API int xdk_kv8_sparse_attention(const void* q, const void* k_cache, const void* v_cache, const float* k_scale, const float* v_scale,
+                             const int32_t* pages, const int64_t* positions, const int64_t* page_table,
+                             const int64_t* sequence_ids, const xdk_peer_out* out_dst, int64_t tokens, int64_t q_heads,
+                             int64_t kv_heads, int64_t head_dim, int64_t max_pages_per_seq, int64_t page_size, int64_t n_pages,
+                             int cache_is_hnd, float scale, int dtype, int codes, unsigned flags, void* stream);
+
+/*
  * Symmetric INT4 quantisation on the device, into the format xdk_w4a16 reads: weight [n, k] row-major of
  * `dtype` (FP32, BF16 or FP16) -> packed uint8 [n, ceil(k/2)] and FP16 scales [n, ceil(k/group_size)].
  * Per (row, group): scale = half(max|w| / 7) (at least 2^-24; 1 for an all-zero group), rounded to FP16
