@@ -54,7 +54,8 @@ SIGNATURES = {
     "xdk_kv8_decode_attention_scratch_bytes": (ctypes.c_size_t, [_i64] * 5),
     "xdk_kv8_decode_attention": (_int, [_p] * 9 + [_i64] * 6 + [_int, ctypes.c_float, _i64, _int, _int, _p, ctypes.c_size_t, _uint, _p]),
     "xdk_kv8_select_pages": (_int, [_p] * 7 + [_i64] * 7 + [_int, _uint, _p]),
-    "xdk_kv8_sparse_attention": (_int, [_p] * 10 + [_i64] * 7 + [_int, ctypes.c_float, _int, _int, _uint, _p]),
+    "xdk_kv8_sparse_attention_scratch_bytes": (ctypes.c_size_t, [_i64] * 6),
+    "xdk_kv8_sparse_attention": (_int, [_p] * 10 + [_i64] * 7 + [_int, ctypes.c_float, _int, _int, _p, ctypes.c_size_t, _uint, _p]),
     "xdk_quantize_int4": (_int, [_p, _int, _i64, _i64, _int, _p, _p, _p, _p]),
     "xdk_peer_fault_flags": (ctypes.c_uint, []),
     "xdk_peer_alloc": (_int, [ctypes.c_size_t, _p]),

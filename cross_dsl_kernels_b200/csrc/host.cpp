@@ -415,13 +415,12 @@ PyObject* kv8_attention(PyObject*, PyObject* const* arg, Py_ssize_t n) {
     c10::cuda::CUDAGuard guard(c.q->device());
     out = at::empty_like(*c.q);
     const size_t need = xdk_kv8_decode_attention_scratch_bytes(c.tokens, c.hq, c.hkv, c.dim, hint);
-    at::Tensor scratch;
-    if (need) scratch = at::empty({static_cast<int64_t>(need)}, c.q->options().dtype(at::kByte));
+    const at::Tensor scratch = at::empty({static_cast<int64_t>(need)}, c.q->options().dtype(at::kByte));
     const xdk_peer_out dst = c.to(out);
     st = xdk_kv8_decode_attention(c.q->data_ptr(), c.k->data_ptr(), c.v->data_ptr(), c.ks->const_data_ptr<float>(), c.vs->const_data_ptr<float>(),
                                   c.pos->const_data_ptr<int64_t>(), c.table->const_data_ptr<int64_t>(), c.seq->const_data_ptr<int64_t>(), &dst,
                                   c.tokens, c.hq, c.hkv, c.dim, c.width, c.page, c.hnd, static_cast<float>(scale), hint, c.code, c.codes,
-                                  need ? scratch.data_ptr() : nullptr, need, launch_flags(dep), stream_of(*c.q));
+                                  scratch.data_ptr(), need, launch_flags(dep), stream_of(*c.q));
   }
   return finish(st, "xdk_kv8_decode_attention", THPVariable_Wrap(std::move(out)));
   END_HANDLE_TH_ERRORS
@@ -467,11 +466,14 @@ PyObject* kv8_sparse(PyObject*, PyObject* const* arg, Py_ssize_t n) {
     Unlocked unlocked;
     c10::cuda::CUDAGuard guard(c.q->device());
     out = at::empty_like(*c.q);
+    const size_t need = xdk_kv8_sparse_attention_scratch_bytes(c.tokens, c.hq, c.hkv, c.dim, c.page, pages->size(2));
+    const at::Tensor scratch = at::empty({static_cast<int64_t>(need)}, c.q->options().dtype(at::kByte));
     const xdk_peer_out dst = c.to(out);
     st = xdk_kv8_sparse_attention(c.q->data_ptr(), c.k->data_ptr(), c.v->data_ptr(), c.ks->const_data_ptr<float>(), c.vs->const_data_ptr<float>(),
                                   pages->const_data_ptr<int32_t>(), c.pos->const_data_ptr<int64_t>(), c.table->const_data_ptr<int64_t>(),
                                   c.seq->const_data_ptr<int64_t>(), &dst, c.tokens, c.hq, c.hkv, c.dim, c.width, c.page, pages->size(2), c.hnd,
-                                  static_cast<float>(scale), c.code, c.codes, launch_flags(dep), stream_of(*c.q));
+                                  static_cast<float>(scale), c.code, c.codes, scratch.data_ptr(), need, launch_flags(dep),
+                                  stream_of(*c.q));
   }
   return finish(st, "xdk_kv8_sparse_attention", THPVariable_Wrap(std::move(out)));
   END_HANDLE_TH_ERRORS

@@ -4,70 +4,116 @@
 // with codes kc, vc and a scale per page and KV head; j runs over 0 .. position, or over those of them that lie in the pages of
 // the token's list.  Nothing to attend to: zeros.
 //
-// Work is dealt out as in the 16-bit read (paged_attention.cuh): CTAs of four warps, a warp takes 32 positions of a tile of 128,
-// K and V rows staged together with cp.async.  A code is exact in FP16, so both contractions are mma.m16n8k16 on FP16 with positions
-// (scores) and dims (values) as the 16 rows and the heads of the group as the 8 columns:
+// A code is exact in FP16, so both contractions are mma.m16n8k16 on FP16 with positions (scores) and dims (values) as the 16 rows and the
+// heads of the group as the 8 columns:
 //   * q is scaled by a power of two, so that its largest value is near 2^14, and rounded to FP16 (FP16 and BF16 values pass whole unless
 //     they are 2^-27 of the largest); an FP32 q is the sum of two such numbers, and each product two products.
-//   * the softmax weights times the block scales, w = p * vs, span any range.  They are taken relative to the running largest of each
-//     head (times 2^14: what rounds away is then below 2^-38 of it), rounded to FP16 (half a step: 2^-12, below the output's 2^-12 or 2^-9), for FP32
-//     again as the sum of two.  The accumulators follow the running largest like the running maximum of the scores.
+//   * the weights are the softmax weights times the block scales of V, w = p * vs = 2^(s + log2 vs): one running maximum, of the whole
+//     exponent, keeps them in range whatever the scales are (down to 2^-90 of the first tile's); the softmax sum takes vs out again.  The largest
+//     weight of a head is 2^14, so that what rounds away is below 2^-38 of it; weights are rounded to FP16 (half a step: 2^-11), for FP32
+//     again as the sum of two.
+//   * int8 codes enter as the subnormal halves (code + 128) * 2^-24, which a byte permute makes; the sums begin with -128 times the sum of
+//     the other operand.  FP32 results would see the few 2^-23 of 128 that this rounds away: for them the codes are centred first.
 //   * a tile's sum is added to the accumulators by FP32 FMAs, with rounding; the tensor core truncates.
 // Bytes of a row come as 16-bit pairs through ldmatrix: for K four dims of a position (q in the same order), for V, transposed, two dims of
 // two positions, which byte permutes sort while they widen the codes.
-#include <cooperative_groups.h>
+//
+// HBM-bound in the long run.  The tiles of 32 positions of all (token, KV head) items stand in one line, and every warp -- a CTA of its own, as
+// many as the SMs hold -- takes an equal range: no barrier but the warp's, and its ring of cp.async stages never runs dry, not at
+// the end of an item either.  Items that several warps share leave one partial result per warp in scratch, which a second launch adds in
+// their order.  (Chunks that the hardware hands out as warps finish, by CTAs or by cancelled launches, measured slower: 70 us against 61
+// for 16 contexts of 8192; a chunk's start costs its warp 6 us without loads.)
 #include <math.h>
 
 #include "kv8.cuh"
-#include "paged_attention.cuh"
-
-namespace cg = cooperative_groups;
+#include "mma_f16.cuh"
 
 namespace xdk {
 namespace {
 
 struct Kv8Args {
-  AttnArgs at;
   const void* q;
   const uint8_t *k_cache, *v_cache;
   const float *k_scale, *v_scale;
+  const int64_t *positions, *page_table, *sequence_ids;
   const int32_t* pages;  // [tokens, kv_heads, n_pages], sparse only
-  int n_pages;
-  int group;  // query heads of a KV head
-  int dtype;  // of q and out
+  float* scratch;
+  int64_t max_pages, page_size;
+  int tokens, q_heads, kv_heads, group;  // group: query heads of a KV head
+  int n_pages, dtype;                    // dtype: of q and out
+  int tile;                              // positions of a tile
+  int hnd, narrow;                       // narrow: every position that a page table row can hold fits 31 bits
+  float scale;
 };
 
-constexpr int kMaxGroup = 8;             // heads of a group: columns of a matrix instruction
-constexpr float kWeightTop = 16384.0f;     // 2^14: the largest weight of a head in FP16
-constexpr float kLeastTop = 7.8886091e-31f;  // 2^-100: weights are not taken relative to less
+constexpr int kMaxGroup = 8;                 // heads of a group: columns of a matrix instruction
+template <int D> constexpr int kTileOf = D == 64 ? 64 : 32;  // positions of a tile: of 8 KB or more
+inline int tile_of(int64_t dim) { return dim == 64 ? kTileOf<64> : kTileOf<128>; }
+constexpr int kEntry = 2;                    // what the change to another item costs a warp, in tiles
+constexpr int kMergeThreads = 256;
+constexpr int64_t kMaxContextHint = 1LL << 38;
+constexpr float kWeightLog2 = 14.0f;            // the largest weight of a head in FP16 is 2^14
+constexpr float kLeastScale = 8.0779357e-28f;   // 2^-90: scales of V below that, in units of the first tile's, count as that
 
-// A warp's stage: K rows, V rows (16-byte pieces xor-swizzled, so that eight rows of an ldmatrix lie on eight bank groups), the
-// scales of the positions, and which of them are alive.
+// A stage: K rows, V rows (16-byte pieces xor-swizzled, so that eight rows of an ldmatrix lie on eight bank groups).
 template <int D>
 struct Stage {
-  static constexpr int kPositions = 32, kStages = D == 256 ? 1 : 2;
-  static constexpr int kRows = kPositions * D;
-  static constexpr int kBytes = 2 * kRows + 2 * kPositions * 4 + 16;
-  static_assert(kMaxGroup * D * 4 <= 2 * kRows, "a warp's accumulators fit the stage that it is done with");
+  static constexpr int kStages = D == 256 ? 1 : 2;
+  static constexpr int kRows = kTileOf<D> * D;
+  static constexpr int kBytes = 2 * kRows;
   __device__ static __forceinline__ int at(int row, int piece) {
     if constexpr (D == 64) return row * D + ((piece ^ (row >> 1 & 3)) << 4);
     return row * D + ((piece ^ (row & 7)) << 4);
   }
 };
-template <int D> constexpr size_t ring_bytes() { return static_cast<size_t>(kAttnWarps) * Stage<D>::kStages * Stage<D>::kBytes; }
+template <int D> constexpr int ring_bytes() { return Stage<D>::kStages * Stage<D>::kBytes; }
 
-__device__ __forceinline__ void cp_async4_or_zero(void* dst_smem, const void* src, bool live) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(dst_smem)), "l"(src), "r"(live ? 4 : 0) : "memory");
-}
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ float load_as_f32(const void* p, int64_t at, int dtype) {
-  if (dtype == XDK_F32) return static_cast<const float*>(p)[at];
-  if (dtype == XDK_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[at]);
-  return __half2float(static_cast<const __half*>(p)[at]);
+__device__ __forceinline__ float log2_fast(float x) {
+  float y;
+  asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// The matrix instructions without `volatile`, so that loads and products of a tile may pass each other; the caller keeps them
+// between its barriers with pin().
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+}
+template <bool TRANS> __device__ __forceinline__ void load_matrices(uint32_t (&r)[4], uint32_t smem_row) {
+  if constexpr (TRANS)
+    asm("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(smem_row));
+  else
+    asm("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(smem_row));
+}
+__device__ __forceinline__ void pin(uint32_t& x) { asm volatile("" : "+r"(x)::"memory"); }
+__device__ __forceinline__ void pin(float& x) { asm volatile("" : "+f"(x)); }
+// Dims 4 quad .. + 3 of each of N pieces of 16, from `at` on.  One type and one branch for all of them, so that the loads go out together.
+template <typename T, int N> __device__ __forceinline__ void load_quads(const T* at, bool vectors, float (&x)[N][4]) {
+  if (vectors) {
+#pragma unroll
+    for (int c = 0; c < N; ++c) {
+      if constexpr (sizeof(T) == 4) {
+        const float4 v = *reinterpret_cast<const float4*>(at + c * 16);
+        x[c][0] = v.x, x[c][1] = v.y, x[c][2] = v.z, x[c][3] = v.w;
+      } else {
+        const uint2 v = *reinterpret_cast<const uint2*>(at + c * 16);
+        const T* e = reinterpret_cast<const T*>(&v);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[c][i] = Elem<T>::to_f32(e[i]);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int c = 0; c < N; ++c)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[c][i] = Elem<T>::to_f32(at[c * 16 + i]);
+  }
 }
 __device__ __forceinline__ void store_from_f32(const PeerOut& out, int64_t row, int64_t col, float v, int dtype) {
   if (dtype == XDK_F32) peer_store(out, row, col, v);
@@ -85,123 +131,235 @@ __device__ __forceinline__ void merge_stats2(float& m_a, float& l_a, float& scal
 // What the sum of the weights divides: nothing was attended to where it is 0.
 __device__ __forceinline__ float normalised(float acc, float l) { return l == 0.0f ? 0.0f : acc / l; }
 
-// Scratch of a grid of `ctas` that split the batch evenly, as in the 16-bit read, for a group of any size.
-struct Kv8Partials {
-  float *acc, *m, *l;  // [2 ctas][group * dim], [2 ctas][group], [2 ctas][group]
-  int* header;         // [ctas][4]
-  __device__ Kv8Partials(float* base, int ctas, int group, int dim) {
-    acc = base;
-    m = acc + static_cast<size_t>(2) * group * dim * ctas;
-    l = m + static_cast<size_t>(2) * group * ctas;
-    header = reinterpret_cast<int*>(l + static_cast<size_t>(2) * group * ctas);
+// ---- the line of tiles ---------------------------------------------------------------------------------------------------
+// Token by token, its KV heads; to each kEntry units and one for every tile of the context (one dead tile for an empty one).  Only the
+// device knows the contexts: each warp adds them up.  Warp b of B has the tiles among units [b U / B, (b + 1) U / B) of the U there are, B:
+// the warps of the grid, or U if that is less.  (Without the entries a warp among contexts of a tile or two had nine of them to begin and
+// to end: 72 us for 64 contexts of 1 .. 2048, where 64 of 1024 took 38.)
+struct Cursor {
+  int token, kvh, tile, tiles;
+  int64_t left;  // units of the warp from this tile on
+};
+template <bool SPARSE> __device__ __forceinline__ int tiles_of(const Kv8Args& a, int64_t context) {
+  if (context <= 0) return 1;
+  return static_cast<int>(((SPARSE ? a.n_pages * a.page_size : context) + a.tile - 1) / a.tile);
+}
+template <bool SPARSE> __device__ __forceinline__ int units_of(const Kv8Args& a, int token) {  // of one of its heads
+  return token < a.tokens ? tiles_of<SPARSE>(a, a.positions[token] + 1) + kEntry : 0;
+}
+// Whole warps call these.
+template <bool SPARSE> __device__ __forceinline__ int64_t count_units(const Kv8Args& a) {
+  int64_t total = 0;
+  for (int t = threadIdx.x; t < a.tokens; t += 32) total += units_of<SPARSE>(a, t);
+#pragma unroll
+  for (int sh = 16; sh > 0; sh >>= 1) total += __shfl_xor_sync(0xffffffffu, total, sh);
+  return total * a.kv_heads;
+}
+// The first tile among units [from, to), whose `left` is 0 if there is none.
+template <bool SPARSE> __device__ __forceinline__ Cursor find_unit(const Kv8Args& a, int64_t from, int64_t to) {
+  const int lane = threadIdx.x;
+  Cursor c = {};
+  int64_t before = 0;
+  for (int t0 = 0; t0 < a.tokens; t0 += 32) {
+    const int units = units_of<SPARSE>(a, t0 + lane);
+    const int64_t mine = static_cast<int64_t>(units) * a.kv_heads;
+    int64_t upto = mine;
+#pragma unroll
+    for (int sh = 1; sh < 32; sh <<= 1) {
+      const int64_t v = __shfl_up_sync(0xffffffffu, upto, sh);
+      if (lane >= sh) upto += v;
+    }
+    const unsigned who = __ballot_sync(0xffffffffu, from < before + upto);
+    if (who != 0) {
+      const int src = __ffs(who) - 1, each = __shfl_sync(0xffffffffu, units, src);
+      const int64_t at = from - before - __shfl_sync(0xffffffffu, upto - mine, src);
+      c.token = t0 + src, c.tiles = each - kEntry;
+      c.kvh = static_cast<int>(at / each);
+      const int in = static_cast<int>(at - static_cast<int64_t>(c.kvh) * each) - kEntry;
+      c.tile = in > 0 ? in : 0;
+      c.left = to - from + (in < 0 ? in : 0);
+      if (c.left < 0) c.left = 0;
+      return c;
+    }
+    before += __shfl_sync(0xffffffffu, upto, 31);
+  }
+  return c;
+}
+// On to the warp's next tile; `context(token)`: what a change of tokens takes.  0: there is none (left is 0), 1: of the same item, 2: of another.
+template <bool SPARSE, typename Context> __device__ __forceinline__ int advance(const Kv8Args& a, Cursor& c, Context context) {
+  ++c.tile, --c.left;
+  if (c.left > 0 && c.tile < c.tiles) return 1;
+  c.left -= kEntry;
+  if (c.left <= 0) {
+    c.left = 0;
+    return 0;
+  }
+  c.tile = 0;
+  if (++c.kvh == a.kv_heads) c.kvh = 0, c.tiles = tiles_of<SPARSE>(a, context(++c.token));
+  return 2;
+}
+
+// Scratch of a grid of `warps`: slot 2 b + 1 is for the item that warp b begins and does not end, slot 2 b for one begun before
+// it.  Accumulators [slots][group * dim], running maxima and sums [slots][8] of each; and for every item the warp that begins it and how
+// many warps have a part of it, which the one that begins it writes.
+struct Partials {
+  float *acc, *m, *l;
+  int2* shares;
+  __device__ Partials(float* scratch, int warps, int values) {
+    acc = scratch;
+    m = acc + static_cast<size_t>(2 * warps) * values;
+    l = m + static_cast<size_t>(2 * warps) * kMaxGroup;
+    shares = reinterpret_cast<int2*>(l + static_cast<size_t>(2 * warps) * kMaxGroup);
   }
 };
+constexpr size_t partial_bytes(size_t warps, size_t items, size_t values) { return 2 * warps * (values + 2 * kMaxGroup) * 4 + items * 8; }
 
 template <typename C, int D, bool SPLIT, bool SPARSE>
-__global__ void __launch_bounds__(kAttnThreads, D <= 128 ? 3 : 2)
-kv8_attention_kernel(const __grid_constant__ Kv8Args p, const __grid_constant__ PeerOut out, int splits) {
+__global__ void __launch_bounds__(32, D == 256 ? 8 : 12)
+kv8_attention_kernel(const __grid_constant__ Kv8Args a, const __grid_constant__ PeerOut out) {
   using St = Stage<D>;
-  constexpr int TP = St::kPositions, PB = TP / 16, NC = D / 16;  // blocks of 16 positions, pieces of 16 dims
-  constexpr int NST = St::kStages, kUnit = kAttnWarps * TP;
-  constexpr int NQ = SPLIT ? 2 : 1;  // FP16 numbers to a value of q or weight
-  extern __shared__ __align__(128) unsigned char smem[];
-  unsigned char* ring = smem + warp_of(threadIdx.x) * NST * St::kBytes;
-  __shared__ float part_m[kAttnWarps][kMaxGroup], part_l[kAttnWarps][kMaxGroup];
-  __shared__ float cta_m[kMaxGroup], cta_l[kMaxGroup];
-  __shared__ int64_t batch_tiles;
-  __shared__ TokenCache cache;
-  const AttnArgs& a = p.at;
+  constexpr int TP = kTileOf<D>, R = TP / 32;  // R: rows that a lane looks up
+  constexpr int PB = TP / 16, NC = D / 16, NST = St::kStages;  // PB: blocks of 16 positions, NC: pieces of 16 dims
+  constexpr int NQ = SPLIT ? 2 : 1;  // FP16 numbers to a value of q (SPLIT: FP32) or weight
+  constexpr bool CENTRED = SPLIT;    // FP32 results would see what an offset of the codes cancels
+  extern __shared__ __align__(128) unsigned char ring[];
+  __shared__ int64_t rows[TP];     // byte offsets of the rows that are fetched
+  __shared__ float4 per_row[TP];   // of a tile's positions: scale of K, log2 of that of V (-infinity: dead), one over it
 
   pdl_launch_dependents();
   pdl_wait();  // q and the caches are the preceding kernels' output
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int lane = threadIdx.x;
   const int grow = lane >> 2, quad = lane & 3;
-  const int G = p.group;
-  const bool even = !SPARSE && a.scratch != nullptr;
-  const int split = even ? 0 : blockIdx.x;
-  ItemCursor cur;  // the tile that is computed next
-  int n_tiles;
-  if (even) {
-    if (threadIdx.x == 0) Kv8Partials(a.scratch, gridDim.x, G, D).header[4 * blockIdx.x] = -1;
-    n_tiles = static_cast<int>(seek_share<kUnit>(a, cur, batch_tiles, cache));
-    if (n_tiles == 0) return;
-  } else {
-    cur.kvh = blockIdx.y, cur.token = blockIdx.z, cur.load<kUnit>(a, nullptr);
-    if constexpr (SPARSE) cur.tiles = cur.ctx > 0 ? static_cast<int>((static_cast<int64_t>(p.n_pages) * a.page_size + kUnit - 1) / kUnit) : 1;
-    cur.tile = static_cast<int>(static_cast<int64_t>(cur.tiles) * split / splits);
-    n_tiles = static_cast<int>(static_cast<int64_t>(cur.tiles) * (split + 1) / splits) - cur.tile;
-  }
-  ItemCursor next = cur;  // the tile whose rows are fetched next
+  const int G = a.group;
+  const int64_t total = count_units<SPARSE>(a), warps = total < gridDim.x ? total : gridDim.x;
+  if (blockIdx.x >= warps) return;
+  const int64_t end_unit = total * (blockIdx.x + 1) / warps;
+  Cursor cur = find_unit<SPARSE>(a, total * blockIdx.x / warps, end_unit);  // the tile that is computed next
+  if (cur.left == 0) return;
+  Cursor next = cur;  // the tile that is fetched next, and what its rows are found by
+  int64_t ctx = 0, coming_ctx = 0, coming_seq = 0;  // of the token, and of the one behind it
+  const int64_t* table = nullptr;
   const int32_t* list = nullptr;
-  if constexpr (SPARSE) list = p.pages + (static_cast<int64_t>(cur.token) * a.kv_heads + cur.kvh) * p.n_pages;
-
-  struct {
-    int64_t page;  // -1: dead
-    int off;
-  } at;  // this lane's row of tile `next`
+  auto glance = [&]() {  // at the token behind
+    if (next.token + 1 < a.tokens) coming_ctx = a.positions[next.token + 1] + 1, coming_seq = a.sequence_ids[next.token + 1];
+  };
+  auto enter = [&](bool other_token) {
+    if (other_token) {
+      ctx = coming_ctx, table = a.page_table + coming_seq * a.max_pages;
+      glance();
+    }
+    if constexpr (SPARSE) list = a.pages + (static_cast<int64_t>(next.token) * a.kv_heads + next.kvh) * a.n_pages;
+    // q of the item, which is loaded when its first tile is computed, on its way to L1
+    const int bytes = G * D * (SPLIT ? 4 : 2);
+    const unsigned char* at = static_cast<const unsigned char*>(a.q) + (static_cast<int64_t>(next.token) * a.q_heads + next.kvh * G) * (D * (SPLIT ? 4 : 2));
+    for (int i = lane * 128; i < bytes; i += 32 * 128) {
+      uint16_t unused;
+      asm volatile("ld.global.u16 %0, [%1];" : "=h"(unused) : "l"(at + i));
+    }
+  };
+  int64_t page[R];  // of this lane's rows of it, -1: dead
+  int off[R];
   auto look_up = [&]() {
-    const int64_t i = static_cast<int64_t>(next.tile) * kUnit + warp * TP + lane;
-    at.page = -1, at.off = 0;
-    if constexpr (!SPARSE) {
-      if (i >= next.ctx) return;
-      const int64_t logical = a.narrow ? static_cast<uint32_t>(i) / static_cast<uint32_t>(a.page_size) : i / a.page_size;
-      at.off = static_cast<int>(i - logical * a.page_size);
-      at.page = next.table[logical];
-    } else {
-      const int entry = static_cast<int>(static_cast<uint32_t>(i) / static_cast<uint32_t>(a.page_size));  // of at most 2^31 positions
-      if (entry >= p.n_pages) return;
-      const int64_t logical = list[entry];
-      // the list ascends: an entry that does not (a second one of a page) is not read
-      if (logical < 0 || (entry > 0 && list[entry - 1] >= logical)) return;
-      at.off = static_cast<int>(i) - entry * static_cast<int>(a.page_size);
-      if (logical * a.page_size + at.off < next.ctx) at.page = next.table[logical];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      page[r] = -1, off[r] = 0;
+      if constexpr (!SPARSE) {
+        const int64_t i = static_cast<int64_t>(next.tile) * TP + r * 32 + lane;
+        if (i < ctx) {
+          const int64_t logical = a.narrow ? static_cast<uint32_t>(i) / static_cast<uint32_t>(a.page_size) : i / a.page_size;
+          off[r] = static_cast<int>(i - logical * a.page_size);
+          page[r] = table[logical];
+        }
+      } else {
+        const uint32_t i = static_cast<uint32_t>(next.tile) * TP + r * 32 + lane;  // of at most 2^31 positions
+        const int entry = static_cast<int>(i / static_cast<uint32_t>(a.page_size));
+        if (entry < a.n_pages && ctx > 0) {
+          const int64_t logical = list[entry];
+          off[r] = static_cast<int>(i) - entry * static_cast<int>(a.page_size);
+          // the list ascends: an entry that does not (a second one of a page) is not read
+          if (logical >= 0 && (entry == 0 || list[entry - 1] < logical) && logical * a.page_size + off[r] < ctx) page[r] = table[logical];
+        }
+      }
     }
   };
-  auto fetch = [&](int stage) {  // tile `next` into a stage, and on to the next one
+  const uint8_t *k_lane = a.k_cache + lane % NC * 16, *v_lane = a.v_cache + lane % NC * 16;
+  float ks[NST][R], vs[NST][R];  // scales of this lane's positions in the tiles on their way, oldest first; -1: dead
+  auto fetch = [&](int stage, float (&k_scale)[R], float (&v_scale)[R]) {  // tile `next` into a stage
     unsigned char* st = ring + stage * St::kBytes;
-    float* scales = reinterpret_cast<float*>(st + 2 * St::kRows);
-    const bool live = at.page >= 0;
-    const unsigned alive = __ballot_sync(0xffffffffu, live);
-    const int64_t row = live ? (a.hnd ? (at.page * a.kv_heads + next.kvh) * a.page_size + at.off
-                                      : (at.page * a.page_size + at.off) * a.kv_heads + next.kvh) * D
-                             : 0;
-    const int64_t block = live ? at.page * a.kv_heads + next.kvh : 0;
-    cp_async4_or_zero(scales + lane, p.k_scale + block, live);
-    cp_async4_or_zero(scales + TP + lane, p.v_scale + block, live);
-    if (lane == 0) *reinterpret_cast<unsigned*>(scales + 2 * TP) = alive;
+    const int kvh = next.kvh;
+    bool all_live = true;
 #pragma unroll
-    for (int i = 0; i < NC; ++i) {  // NC pieces to a row
-      const int c = i * 32 + lane, r = c / NC, piece = c - r * NC;
-      const int64_t from = __shfl_sync(0xffffffffu, row, r) + piece * 16;
-      const bool there = alive >> r & 1u;
-      cp_async16_or_zero(st + St::at(r, piece), p.k_cache + from, there);
-      cp_async16_or_zero(st + St::kRows + St::at(r, piece), p.v_cache + from, there);
+    for (int r = 0; r < R; ++r) {
+      const bool live = page[r] >= 0;
+      all_live = all_live && live;
+      const int64_t block = live ? page[r] * a.kv_heads + kvh : 0;
+      rows[r * 32 + lane] = live ? (a.hnd ? block * a.page_size + off[r] : (page[r] * a.page_size + off[r]) * a.kv_heads + kvh) * D : -1;
+      k_scale[r] = live ? a.k_scale[block] : 0.0f;
+      v_scale[r] = live ? a.v_scale[block] : -1.0f;
     }
+    constexpr int kAtOnce = 32 / NC;  // rows of NC pieces
+    if (__all_sync(0xffffffffu, all_live)) {
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < TP / kAtOnce; ++i) {
+        const int r = i * kAtOnce + lane / NC;
+        const int64_t from = rows[r];
+        cp_async16(st + St::at(r, lane % NC), k_lane + from);
+        cp_async16(st + St::kRows + St::at(r, lane % NC), v_lane + from);
+      }
+    } else {
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < TP / kAtOnce; ++i) {
+        const int r = i * kAtOnce + lane / NC;
+        const int64_t from = rows[r];
+        const bool there = from >= 0;
+        cp_async16_or_zero(st + St::at(r, lane % NC), k_lane + (there ? from : 0), there);
+        cp_async16_or_zero(st + St::kRows + St::at(r, lane % NC), v_lane + (there ? from : 0), there);
+      }
+    }
+    __syncwarp();  // rows is free again
   };
-  auto step = [&](ItemCursor& c) {
-    if (even) c.advance<kUnit>(a, &cache);
-    else ++c.tile;
+  auto fetch_next = [&](int stage, float (&k_scale)[R], float (&v_scale)[R]) {  // one group per call, whether or not there is a tile left
+    if (next.left > 0) {
+      fetch(stage, k_scale, v_scale);
+      const int step = advance<SPARSE>(a, next, [&](int) { return coming_ctx; });
+      if (step == 2) enter(next.kvh == 0);
+      if (step != 0) look_up();  // the page of the row after that is on its way meanwhile
+    }
+    cp_async_commit();
   };
+  coming_ctx = a.positions[next.token] + 1, coming_seq = a.sequence_ids[next.token];
+  enter(true);
+  look_up();
+#pragma unroll
+  for (int s = 0; s < NST - 1; ++s) fetch_next(s, ks[s], vs[s]);
+  const uint32_t ring_at = smem_u32(ring);
+  int stage = 0;
 
-  uint32_t qb[NQ][NC][2];    // q^T as B fragments: dims 16 c + 4 quad + {0,1}, {2,3} of head grow
-  float unit[2];             // of the scores of heads 2 quad + {0, 1}: scale * log2(e) * the power of two that q was divided by
-  float m_run[2], l_run[2];  // of these heads; l_run is this thread's share of the sum
-  float w_top[2];            // the largest weight of these heads so far, as of m_run
-  float o[NC][4];            // O^T: dims 16 c + 2 grow (+ 1 in the upper two), heads 2 quad + {0, 1}; in units of w_top / kWeightTop
-  auto begin_segment = [&](int token, int kvh) {
-#pragma unroll
-    for (int e = 0; e < 2; ++e) m_run[e] = -INFINITY, l_run[e] = 0.0f, w_top[e] = 0.0f;
-#pragma unroll
-    for (int c = 0; c < NC; ++c)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) o[c][e] = 0.0f;
-    const bool head_live = grow < G;
+  for (;;) {  // the warp's part of one item after the other
+  const int token = cur.token, kvh = cur.kvh, first = cur.tile;
+  const int end = cur.tiles - first < cur.left ? cur.tiles : first + static_cast<int>(cur.left);
+  float x[NC][4];  // q: dims 16 c + 4 quad .. of head grow
+  const bool head_live = grow < G;
+  {
     const int64_t qrow = (static_cast<int64_t>(token) * a.q_heads + kvh * G + (head_live ? grow : 0)) * D + quad * 4;
+    const bool vectors = (reinterpret_cast<uintptr_t>(a.q) & 15) == 0;
+    if constexpr (SPLIT) load_quads(static_cast<const float*>(a.q) + qrow, vectors, x);
+    else if (a.dtype == XDK_BF16) load_quads(static_cast<const __nv_bfloat16*>(a.q) + qrow, vectors, x);
+    else load_quads(static_cast<const __half*>(a.q) + qrow, vectors, x);
+  }
+  uint32_t qb[NQ][NC][2];  // q^T as B fragments: dims 16 c + 4 quad + {0,1}, {2,3} of head grow
+  float unit[2];           // of the scores of heads 2 quad + {0, 1}: scale * log2(e) * the power of two that q was divided by
+  {
     float top = 0.0f;
 #pragma unroll
     for (int c = 0; c < NC; ++c)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) top = fmaxf(top, head_live ? fabsf(load_as_f32(p.q, qrow + c * 16 + e, p.dtype)) : 0.0f);
+      for (int e = 0; e < 4; ++e) {
+        if (!head_live) x[c][e] = 0.0f;
+        top = fmaxf(top, fabsf(x[c][e]));
+      }
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
     const int exponent = static_cast<int>(__float_as_uint(top) >> 23) - 127;
@@ -212,178 +370,148 @@ kv8_attention_kernel(const __grid_constant__ Kv8Args p, const __grid_constant__ 
     for (int c = 0; c < NC; ++c)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        float x[2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) x[e] = head_live ? load_as_f32(p.q, qrow + c * 16 + 2 * h + e, p.dtype) * by : 0.0f;
-        const __half2 hi = __floats2half2_rn(x[0], x[1]);
+        const float x0 = x[c][2 * h] * by, x1 = x[c][2 * h + 1] * by;
+        const __half2 hi = __floats2half2_rn(x0, x1);
         qb[0][c][h] = *reinterpret_cast<const uint32_t*>(&hi);
         if constexpr (SPLIT) {
           const float2 f = __half22float2(hi);
-          qb[NQ - 1][c][h] = Mma16816<__half>::pack(x[0] - f.x, x[1] - f.y);
+          qb[NQ - 1][c][h] = Mma16816<__half>::pack(x0 - f.x, x1 - f.y);
         }
       }
 #pragma unroll
-    for (int e = 0; e < 2; ++e) unit[e] = __shfl_sync(0xffffffffu, back, (2 * quad + e) * 4) * (a.scale * 1.4426950408889634f);
-  };
-  // a warp's accumulators [group * D], in a stage that it is done with
-  auto acc_of = [&](int w, int done) { return reinterpret_cast<float*>(smem + (w * NST + done) * St::kBytes); };
-  auto write_partials = [&](int done) {  // of this warp
+    for (int e = 0; e < 2; ++e)
+      unit[e] = __shfl_sync(0xffffffffu, back, (2 * quad + e) * 4) * (a.scale * 1.4426950408889634f / (CENTRED ? 1.0f : Codec<C>::kUnit));
+  }
+  float s_zero[2] = {0.0f, 0.0f};  // what a score begins with: codes that are not centred add kOffset * q
+  if constexpr (!CENTRED && Codec<C>::kOffset != 0.0f) {
+    float sum = 0.0f;
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
+    for (int c = 0; c < NC; ++c)
 #pragma unroll
-      for (int sh = 4; sh < 32; sh <<= 1) l_run[e] += __shfl_xor_sync(0xffffffffu, l_run[e], sh);
-      const int head = quad * 2 + e;
-      if (head < G) {
-        if (grow == 0) part_m[warp][head] = m_run[e], part_l[warp][head] = l_run[e];
-        const float back = w_top[e] * (1.0f / kWeightTop);
-        float* to = acc_of(warp, done) + head * D + 2 * grow;
+      for (int h = 0; h < 2; ++h) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&qb[0][c][h]));
+        sum += f.x + f.y;
+      }
+    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
 #pragma unroll
-        for (int c = 0; c < NC; ++c) *reinterpret_cast<float2*>(to + c * 16) = make_float2(o[c][e] * back, o[c][e + 2] * back);
-      }
-    }
-  };
-  // The four warps' partial results -> the output, when the CTA has the whole item, or this CTA's slot of scratch.
-  auto finish_segment = [&](int done, int token, int kvh, int tiles_left, bool begins) {
-    __syncthreads();
-    const Kv8Partials part(a.scratch, gridDim.x, G, D);
-    const int slot = 2 * blockIdx.x + (begins ? 1 : 0);
-    const bool ends = tiles_left == 0;  // of the item, behind this segment
-    if (begins && !ends && threadIdx.x == 0) {
-      // the CTA that holds the item's last tile: the tile's number in the batch is this CTA's last one + what is left
-      const int64_t ctas = share_ctas(batch_tiles), last = batch_tiles * (blockIdx.x + 1) / ctas + tiles_left - 1;
-      int* h = part.header + 4 * blockIdx.x;
-      h[0] = token, h[1] = kvh, h[2] = static_cast<int>(((last + 1) * ctas - 1) / batch_tiles);
-    }
-    for (int i = threadIdx.x; i < G * D; i += kAttnThreads) {
-      const int g = i / D, d = i - g * D;
-      float mm = part_m[0][g], ll = part_l[0][g], aa = acc_of(0, done)[i];
-      for (int w = 1; w < kAttnWarps; ++w) {
-        float sa, sb;
-        merge_stats2(mm, ll, sa, sb, part_m[w][g], part_l[w][g]);
-        aa = aa * sa + acc_of(w, done)[i] * sb;
-      }
-      if (begins && ends) {
-        store_from_f32(out, token, (kvh * G + g) * D + d, normalised(aa, ll), p.dtype);
-      } else {
-        part.acc[static_cast<size_t>(slot) * G * D + i] = aa;
-        if (d == 0) part.m[slot * G + g] = mm, part.l[slot * G + g] = ll;
-      }
-    }
-    __syncthreads();
-  };
+    for (int e = 0; e < 2; ++e) s_zero[e] = -Codec<C>::kOffset * Codec<C>::kUnit * __shfl_sync(0xffffffffu, sum, (2 * quad + e) * 4);
+  }
+  // Of heads 2 quad + {0, 1}: the running maximum of s + log2(scale of V), in units of log2 -- what makes the largest weight 2^14 --, and
+  // this thread's share of the sum of the softmax weights, which lack the scale.
+  float m_run[2], l_run[2];
+  float o[NC][4];  // O^T: dims 16 c + 2 grow (+ 1 in the upper two), the same heads
+#pragma unroll
+  for (int e = 0; e < 2; ++e) m_run[e] = -INFINITY, l_run[e] = 0.0f;
+#pragma unroll
+  for (int c = 0; c < NC; ++c)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[c][e] = 0.0f;
+  float v_unit = 0.0f;  // scales of V are taken in units of the largest of the first tile
 
-  int fetched = 0;
-  if (n_tiles > 0) look_up();
-  auto fetch_next = [&](int stage) {  // one group per call, whether or not there is a tile left
-    if (fetched < n_tiles) {
-      fetch(stage);
-      if (++fetched < n_tiles) {  // the page of the row after that is on its way meanwhile
-        step(next);
-        look_up();
-      }
-    }
-    cp_async_commit();
-  };
+  // rows pb * 16 + lane % 16, pieces c + lane / 16 of an even c: offsets that the stage and pb are added to
+  uint32_t at_piece[NC / 2];
 #pragma unroll
-  for (int s = 0; s < NST - 1; ++s) fetch_next(s);
-  bool fresh = true;    // the tile begins a segment
-  bool begins = false;  // the segment begins at its item's first tile
-  if (n_tiles == 0) begin_segment(cur.token, cur.kvh);  // a split without tiles contributes nothing
+  for (int c = 0; c < NC; c += 2) at_piece[c / 2] = St::at(lane & 15, c + (lane >> 4));
 
-  int stage = 0;
-  for (int u = 0; u < n_tiles; ++u) {
-    fetch_next(stage == 0 ? NST - 1 : stage - 1);
-    if (fresh) {
-      begin_segment(cur.token, cur.kvh);
-      begins = cur.tile == 0;
+  for (int u = first; u < end; ++u) {
+    fetch_next(stage == 0 ? NST - 1 : stage - 1, ks[NST - 1], vs[NST - 1]);
+    if (u == first) {
+      v_unit = vs[0][0];
+#pragma unroll
+      for (int r = 1; r < R; ++r) v_unit = fmaxf(v_unit, vs[0][r]);
+#pragma unroll
+      for (int sh = 16; sh > 0; sh >>= 1) v_unit = fmaxf(v_unit, __shfl_xor_sync(0xffffffffu, v_unit, sh));
+      if (!(v_unit > 1e-37f)) v_unit = 1.0f;
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const bool live = !(vs[0][r] < 0.0f);  // NaN is alive
+      float rel = __fdividef(vs[0][r], v_unit);
+      rel = rel < kLeastScale ? kLeastScale : rel;  // NaN passes
+      const float in_exponent = log2_fast(rel);
+      per_row[r * 32 + lane] = make_float4(ks[0][r], live ? in_exponent : -INFINITY, live ? exp2_fast(-in_exponent) : 0.0f, 0.0f);
+#pragma unroll
+      for (int s = 0; s < NST - 1; ++s) ks[s][r] = ks[s + 1][r], vs[s][r] = vs[s + 1][r];
     }
     cp_async_wait<NST - 1>();
     __syncwarp();
-    const unsigned char* ktile = ring + stage * St::kBytes;
-    const unsigned char* vtile = ktile + St::kRows;
-    const float* scales = reinterpret_cast<const float*>(ktile + 2 * St::kRows);
-    const unsigned alive = *reinterpret_cast<const unsigned*>(scales + 2 * TP);
+    uint32_t kt = ring_at + stage * St::kBytes;
+    pin(kt);
+    const uint32_t vt = kt + St::kRows;
 
     // ---- S^T = K q^T: per load, rows 0-7 and 8-15 of a block and two pieces
     float sc[PB][4];  // positions 16 pb + grow (+ 8 in the upper two), heads 2 quad + {0, 1}
 #pragma unroll
     for (int pb = 0; pb < PB; ++pb)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) sc[pb][e] = 0.0f;
+      for (int e = 0; e < 4; ++e) sc[pb][e] = s_zero[e & 1];
 #pragma unroll
     for (int c = 0; c < NC; c += 2)
 #pragma unroll
       for (int pb = 0; pb < PB; ++pb) {
         uint32_t raw[4];
-        ldmatrix_x4(raw, ktile + St::at(pb * 16 + (lane & 15), c + (lane >> 4)));
+        load_matrices<false>(raw, kt + at_piece[c / 2] + pb * 16 * D);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           uint32_t k[4];
-          Codec<C>::neighbours(raw[2 * h], k[0], k[2]);
-          Codec<C>::neighbours(raw[2 * h + 1], k[1], k[3]);
+          Codec<C>::template neighbours<CENTRED>(raw[2 * h], k[0], k[2]);
+          Codec<C>::template neighbours<CENTRED>(raw[2 * h + 1], k[1], k[3]);
 #pragma unroll
-          for (int n = 0; n < NQ; ++n) Mma16816<__half>::run(sc[pb], k, qb[n][c + h][0], qb[n][c + h][1]);
+          for (int n = 0; n < NQ; ++n) mma(sc[pb], k, qb[n][c + h]);
         }
       }
-    // ---- online softmax of the two heads, in units of log2; weights relative to the largest
-    float mx[2] = {-INFINITY, -INFINITY}, vs[PB][2];
+    // ---- online softmax of the two heads.  With the scale of V in the exponent the weights have one running maximum; the sum
+    // takes the scale out again.
+    float mx[2] = {m_run[0], m_run[1]}, take_out[PB][2];
 #pragma unroll
     for (int pb = 0; pb < PB; ++pb)
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        const int j = pb * 16 + grow + r * 8;
-        const float ks = scales[j];
-        vs[pb][r] = scales[TP + j];
-        const bool live = alive >> j & 1u;
+        const float4 f = per_row[pb * 16 + grow + r * 8];
+        take_out[pb][r] = f.z;
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           float& s = sc[pb][2 * r + e];
-          s = live ? s * (ks * unit[e]) : -INFINITY;
+          s = fmaf(s, f.x * unit[e], f.y);
           mx[e] = fmaxf(mx[e], s);
         }
       }
-    float corr[2], wt[2] = {0.0f, 0.0f};
+    float corr[2], from[2];
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
 #pragma unroll
       for (int sh = 4; sh < 32; sh <<= 1) mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], sh));
-      const float m_new = fmaxf(m_run[e], mx[e]);
-      corr[e] = m_run[e] == -INFINITY ? 0.0f : exp2_fast(m_run[e] - m_new);
-      m_run[e] = m_new;
+      from[e] = mx[e] == -INFINITY ? 0.0f : mx[e] - kWeightLog2;
+      corr[e] = exp2_fast(m_run[e] - mx[e]);
+      if (mx[e] == -INFINITY) corr[e] = 1.0f;  // nothing yet
+      m_run[e] = mx[e];
       l_run[e] *= corr[e];
     }
-#pragma unroll
-    for (int pb = 0; pb < PB; ++pb)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float pr = sc[pb][e] == -INFINITY ? 0.0f : exp2_fast(sc[pb][e] - m_run[e & 1]);
-        l_run[e & 1] += pr;
-        sc[pb][e] = pr * vs[pb][e >> 1];
-        wt[e & 1] = fmaxf(wt[e & 1], fabsf(sc[pb][e]));
-      }
-    float rel[2];
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-#pragma unroll
-      for (int sh = 4; sh < 32; sh <<= 1) wt[e] = fmaxf(wt[e], __shfl_xor_sync(0xffffffffu, wt[e], sh));
-      const float was = w_top[e] * corr[e];
-      w_top[e] = fmaxf(fmaxf(was, wt[e]), kLeastTop);
-      rel[e] = __fdividef(kWeightTop, w_top[e]);
-      corr[e] = was * (rel[e] * (1.0f / kWeightTop));
-    }
     uint32_t wb[NQ][PB][2];  // w^T as B fragments: positions 16 pb + 2 quad + {0,1} (+ 8 in [1]), head grow
+    float t_zero[2] = {0.0f, 0.0f};  // as s_zero: kOffset * the tile's weights
 #pragma unroll
     for (int pb = 0; pb < PB; ++pb)
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        const float x0 = sc[pb][2 * r] * rel[0], x1 = sc[pb][2 * r + 1] * rel[1];
+        const float x0 = exp2_fast(sc[pb][2 * r] - from[0]), x1 = exp2_fast(sc[pb][2 * r + 1] - from[1]);
+        l_run[0] = fmaf(x0, take_out[pb][r], l_run[0]), l_run[1] = fmaf(x1, take_out[pb][r], l_run[1]);
         const __half2 hi = __floats2half2_rn(x0, x1);
         wb[0][pb][r] = transpose8x8(*reinterpret_cast<const uint32_t*>(&hi));
-        if constexpr (SPLIT) {
+        if constexpr (SPLIT || Codec<C>::kOffset != 0.0f) {
           const float2 f = __half22float2(hi);
-          wb[NQ - 1][pb][r] = transpose8x8(Mma16816<__half>::pack(x0 - f.x, x1 - f.y));
+          if constexpr (SPLIT) wb[NQ - 1][pb][r] = transpose8x8(Mma16816<__half>::pack(x0 - f.x, x1 - f.y));
+          else t_zero[0] += f.x, t_zero[1] += f.y;
         }
       }
+    if constexpr (!CENTRED && Codec<C>::kOffset != 0.0f) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+#pragma unroll
+        for (int sh = 4; sh < 32; sh <<= 1) t_zero[e] += __shfl_xor_sync(0xffffffffu, t_zero[e], sh);
+        t_zero[e] *= -Codec<C>::kOffset * Codec<C>::kUnit;
+      }
+    }
     // ---- O^T += V^T w^T: per load, position halves of a block and two pieces
 #pragma unroll
     for (int c = 0; c < NC; c += 2) {
@@ -391,173 +519,149 @@ kv8_attention_kernel(const __grid_constant__ Kv8Args p, const __grid_constant__ 
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) t[h][e] = 0.0f;
+        for (int e = 0; e < 4; ++e) t[h][e] = t_zero[e & 1];
 #pragma unroll
       for (int pb = 0; pb < PB; ++pb) {
         uint32_t raw[4];
-        ldmatrix_x4_trans(raw, vtile + St::at(pb * 16 + (lane & 15), c + (lane >> 4)));
+        load_matrices<true>(raw, vt + at_piece[c / 2] + pb * 16 * D);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           uint32_t v[4];
-          Codec<C>::alternate(raw[2 * h], v[0], v[1]);
-          Codec<C>::alternate(raw[2 * h + 1], v[2], v[3]);
+          Codec<C>::template alternate<CENTRED>(raw[2 * h], v[0], v[1]);
+          Codec<C>::template alternate<CENTRED>(raw[2 * h + 1], v[2], v[3]);
 #pragma unroll
-          for (int n = 0; n < NQ; ++n) Mma16816<__half>::run(t[h], v, wb[n][pb][0], wb[n][pb][1]);
+          for (int n = 0; n < NQ; ++n) mma(t[h], v, wb[n][pb]);
         }
       }
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[c + h][e] = fmaf(o[c + h][e], corr[e & 1], t[h][e]);
+        for (int e = 0; e < 4; ++e) {
+          o[c + h][e] = fmaf(o[c + h][e], corr[e & 1], t[h][e]);
+          pin(o[c + h][e]);
+        }
     }
     __syncwarp();  // every lane has read the tile
-    const int done = stage;
     stage = stage + 1 == NST ? 0 : stage + 1;
-
-    const int tiles_left = cur.tiles - 1 - cur.tile;
-    fresh = even && (tiles_left == 0 || u + 1 == n_tiles);
-    if (fresh) {
-      write_partials(done);
-      finish_segment(done, cur.token, cur.kvh, tiles_left, begins);
-    }
-    if (u + 1 < n_tiles) step(cur);
   }
-  if (even) return;
 
-  // ---- grid of splits: warp totals, then the four warps of the CTA (fixed order), then the cluster
-  const int token = cur.token, kvh = cur.kvh;
-  write_partials(0);
-  float* accs = acc_of(0, 0);
-  __syncthreads();
-  for (int i = threadIdx.x; i < G * D; i += kAttnThreads) {
-    const int g = i / D, d = i - g * D;
-    float mm = part_m[0][g], ll = part_l[0][g], aa = accs[i];
-    for (int w = 1; w < kAttnWarps; ++w) {
-      float sa, sb;
-      merge_stats2(mm, ll, sa, sb, part_m[w][g], part_l[w][g]);
-      aa = aa * sa + acc_of(w, 0)[i] * sb;
-    }
-    accs[i] = aa;
-    if (d == 0) cta_m[g] = mm, cta_l[g] = ll;
+  // ---- the result, or this warp's share of it
+  const bool whole = first == 0 && end == cur.tiles;
+  const Partials part(a.scratch, gridDim.x, G * D);
+  const size_t slot = 2 * static_cast<size_t>(blockIdx.x) + (first == 0 ? 1 : 0);
+  if (first == 0 && lane == 0) {  // an item that others go on with ends cur.tiles - end units behind this warp's share
+    const int last = whole ? blockIdx.x : static_cast<int>(((end_unit + cur.tiles - end) * warps - 1) / total);
+    part.shares[static_cast<int64_t>(token) * a.kv_heads + kvh] = make_int2(blockIdx.x, last - blockIdx.x + 1);
   }
-  __syncthreads();
-  if (splits > 1) {
-    cg::cluster_group cluster = cg::this_cluster();
-    cluster.sync();  // every slice's partial is in its CTA's shared memory
-    if (split == 0) {
-      for (int i = threadIdx.x; i < G * D; i += kAttnThreads) {
-        const int g = i / D, d = i - g * D;
-        float mm = cta_m[g], ll = cta_l[g], aa = accs[i];
-        for (int r = 1; r < splits; ++r) {  // rank order
-          const float mr = *cluster.map_shared_rank(&cta_m[g], r), lr = *cluster.map_shared_rank(&cta_l[g], r);
-          const float ar = *cluster.map_shared_rank(&accs[i], r);
-          float sa, sb;
-          merge_stats2(mm, ll, sa, sb, mr, lr);
-          aa = aa * sa + ar * sb;
-        }
-        store_from_f32(out, token, (kvh * G + g) * D + d, normalised(aa, ll), p.dtype);
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+#pragma unroll
+    for (int sh = 4; sh < 32; sh <<= 1) l_run[e] += __shfl_xor_sync(0xffffffffu, l_run[e], sh);
+    const int head = quad * 2 + e;
+    if (head >= G) continue;
+    const float back = v_unit / (CENTRED ? 1.0f : Codec<C>::kUnit);
+    if (whole) {
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          store_from_f32(out, token, (kvh * G + head) * D + c * 16 + 2 * grow + i, normalised(o[c][e + 2 * i] * back, l_run[e]), a.dtype);
+    } else {
+      float* to = part.acc + (slot * G + head) * D + 2 * grow;
+#pragma unroll
+      for (int c = 0; c < NC; ++c) *reinterpret_cast<float2*>(to + c * 16) = make_float2(o[c][e] * back, o[c][e + 2] * back);
+      if (grow == 0) {
+        part.m[slot * kMaxGroup + head] = m_run[e];
+        part.l[slot * kMaxGroup + head] = l_run[e];
       }
     }
-    cluster.sync();  // nobody leaves while rank 0 may still read its shared memory
-  } else {
-    for (int i = threadIdx.x; i < G * D; i += kAttnThreads) {
-      const int g = i / D, d = i - g * D;
-      store_from_f32(out, token, (kvh * G + g) * D + d, normalised(accs[i], cta_l[g]), p.dtype);
-    }
+  }
+  cur.left -= end - 1 - first, cur.tile = end - 1;
+  if (advance<SPARSE>(a, cur, [&](int t) { return a.positions[t] + 1; }) == 0) return;
   }
 }
 
-// Block b adds the partial results of the item that CTA b began and others went on with, a thread four head dims, in CTA order.
+// Adds the parts of one item: L lanes of four values each to a CTA, the threads / L groups of them every so many parts; the groups' sums meet
+// in shared memory.  Always in the same order.  L: a warp where there are few items, so that many CTAs share an item; else what the
+// group * dim values take, at most all threads.
+template <int L>
 __global__ void __launch_bounds__(kMergeThreads)
-kv8_attention_merge_kernel(const __grid_constant__ PeerOut out, float* scratch, int group, int dim, int dtype) {
+kv8_attention_merge_kernel(const __grid_constant__ Kv8Args a, const __grid_constant__ PeerOut out, int dim, int grid) {
+  constexpr int kGroups = kMergeThreads / L;
+  __shared__ float4 accs[kGroups][L];
+  __shared__ float ms[kGroups][L], ls[kGroups][L];
   pdl_launch_dependents();
   pdl_wait();
-  const int b = blockIdx.x;
-  const Kv8Partials p(scratch, gridDim.x, group, dim);
-  const int4 h = __ldcg(reinterpret_cast<const int4*>(p.header + 4 * b));
-  if (h.x < 0) return;
-  const int count = h.z - b + 1, all = group * dim / 4;
-  for (int l4 = threadIdx.x; l4 < all; l4 += kMergeThreads) {
-    const int g = l4 * 4 / dim;
-    float m = -INFINITY, l = 0.0f;
-    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-    for (int i = 0; i < count; ++i) {
-      const int slot = i == 0 ? 2 * b + 1 : 2 * (b + i);
-      const float4 v = __ldcg(reinterpret_cast<const float4*>(p.acc) + static_cast<size_t>(slot) * all + l4);
-      float sa, sb;
-      merge_stats2(m, l, sa, sb, __ldcg(p.m + slot * group + g), __ldcg(p.l + slot * group + g));
-      acc.x = acc.x * sa + v.x * sb, acc.y = acc.y * sa + v.y * sb;
-      acc.z = acc.z * sa + v.z * sb, acc.w = acc.w * sa + v.w * sb;
-    }
-    const int col = h.y * group * dim + l4 * 4;
-    store_from_f32(out, h.x, col, normalised(acc.x, l), dtype);
-    store_from_f32(out, h.x, col + 1, normalised(acc.y, l), dtype);
-    store_from_f32(out, h.x, col + 2, normalised(acc.z, l), dtype);
-    store_from_f32(out, h.x, col + 3, normalised(acc.w, l), dtype);
+  const int group = threadIdx.x / L, lane = threadIdx.x - group * L;
+  const int all = a.group * dim, at = (blockIdx.y * L + lane) * 4;  // dim is a multiple of 64: four values of one head
+  const Partials part(a.scratch, grid, all);
+  const int2 share = __ldcg(part.shares + blockIdx.x);
+  if (share.y == 1) return;  // the same for all threads
+  const bool some = at < all;
+  const int head = some ? at / dim : 0;
+  float m = -INFINITY, l = 0.0f;
+  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  auto add = [&](const float4& v, float mv, float lv) {
+    float sa, sb;
+    merge_stats2(m, l, sa, sb, mv, lv);
+    acc.x = acc.x * sa + v.x * sb, acc.y = acc.y * sa + v.y * sb;
+    acc.z = acc.z * sa + v.z * sb, acc.w = acc.w * sa + v.w * sb;
+  };
+#pragma unroll 8
+  for (int i = group; i < share.y; i += kGroups) {
+    const size_t slot = 2 * static_cast<size_t>(share.x + i) + (i == 0 ? 1 : 0);
+    const float4 v = some ? __ldcg(reinterpret_cast<const float4*>(part.acc + slot * all + at)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    add(v, __ldcg(part.m + slot * kMaxGroup + head), __ldcg(part.l + slot * kMaxGroup + head));
   }
+  if constexpr (kGroups > 1) {
+    accs[group][lane] = acc, ms[group][lane] = m, ls[group][lane] = l;
+    __syncthreads();
+    if (group != 0) return;
+    for (int w = 1; w < kGroups; ++w) add(accs[w][lane], ms[w][lane], ls[w][lane]);
+  }
+  if (!some) return;
+  const int token = blockIdx.x / a.kv_heads, kvh = blockIdx.x - token * a.kv_heads;
+  const int64_t col = static_cast<int64_t>(kvh) * all + at;
+  store_from_f32(out, token, col, normalised(acc.x, l), a.dtype);
+  store_from_f32(out, token, col + 1, normalised(acc.y, l), a.dtype);
+  store_from_f32(out, token, col + 2, normalised(acc.z, l), a.dtype);
+  store_from_f32(out, token, col + 3, normalised(acc.w, l), a.dtype);
 }
 
-inline size_t cta_smem(int64_t dim) { return dim == 64 ? ring_bytes<64>() : (dim == 128 ? ring_bytes<128>() : ring_bytes<256>()); }
-// CTAs that an SM holds: by the shared memory (with what they have statically and what is reserved) and by the kernel's launch bounds
-inline int64_t resident(int64_t dim) {
-  const int64_t by_smem = static_cast<int64_t>((227 * 1024) / (cta_smem(dim) + 4096)), by_regs = dim <= 128 ? 3 : 2;
-  return by_smem < 1 ? 1 : (by_smem < by_regs ? by_smem : by_regs);
+// ---- host --------------------------------------------------------------------------------------------------------------
+
+// Warps of a launch: what the SMs hold at once, by the shared memory of a CTA (and 1 KB reserved) and the launch bounds, and no more than
+// leaves every one as many tiles as the busiest has anyway, if no context has more than `tiles`.
+int grid_for(int64_t items, int64_t dim, int64_t tiles) {
+  const int ring = (dim == 64 ? ring_bytes<64>() : (dim == 128 ? ring_bytes<128>() : ring_bytes<256>())) + tile_of(dim) * 24 + 1024;
+  const int by_smem = 228 * 1024 / ring, by_regs = dim == 256 ? 8 : 12;
+  const int64_t most = static_cast<int64_t>(by_smem < by_regs ? by_smem : by_regs) * sm_count();
+  if (tiles > most) return static_cast<int>(most);
+  const int64_t all = items * ((tiles < 1 ? 1 : tiles) + kEntry), warps = all < most ? all : most, each = (all + warps - 1) / warps;
+  return static_cast<int>((all + each - 1) / each);
 }
-// CTAs of a launch that splits the batch evenly (0: the batch stays on the grid of splits), as in the 16-bit read.
-inline int kv8_even_grid(int64_t tokens, int64_t kv_heads, int64_t dim, int64_t hint) {
-  if (tokens > kMaxTokensSplit || hint < kMinEvenContext) return 0;
-  int64_t ctas = resident(dim) * sm_count();
-  const int64_t most = tokens * kv_heads * ((hint + kAttnThreads - 1) / kAttnThreads);  // tiles
-  if (most < ctas) ctas = most;
-  const int64_t each = (most + ctas - 1) / ctas;
-  return static_cast<int>((most + each - 1) / each);
-}
+int64_t hint_tiles(int64_t context, int64_t dim) { return ((context < 1 ? kMaxContextHint : context) + tile_of(dim) - 1) / tile_of(dim); }
 
 template <typename C, int D, bool SPLIT, bool SPARSE>
-int launch_kv8(const Kv8Args& p, const PeerOut& out, int splits, cudaStream_t s) {
-  const AttnArgs& a = p.at;
-  auto kernel = kv8_attention_kernel<C, D, SPLIT, SPARSE>;
-  const size_t smem = cta_smem(D);
-  if (smem > 40 * 1024) {
-    const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-    if (err != cudaSuccess) return note_launch(err);
-  }
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = a.scratch ? dim3(static_cast<unsigned>(splits))
-                          : dim3(static_cast<unsigned>(splits), static_cast<unsigned>(a.kv_heads), static_cast<unsigned>(a.tokens));
-  cfg.blockDim = dim3(kAttnThreads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = s;
-  cudaLaunchAttribute attr[2];
-  unsigned n = 0;
-  if (splits > 1 && !a.scratch) {
-    attr[n].id = cudaLaunchAttributeClusterDimension;
-    attr[n].val.clusterDim.x = static_cast<unsigned>(splits);
-    attr[n].val.clusterDim.y = 1;
-    attr[n].val.clusterDim.z = 1;
-    ++n;
-  }
-  if (call_flags() & XDK_DEPENDENT_LAUNCH) {
-    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[n].val.programmaticStreamSerializationAllowed = 1;
-    ++n;
-  }
-  cfg.attrs = attr;
-  cfg.numAttrs = n;
-  const int st = note_launch(cudaLaunchKernelEx(&cfg, kernel, p, out, splits));
-  if (st != XDK_OK || !a.scratch) return st;
-  return launch_opts(kv8_attention_merge_kernel, dim3(static_cast<unsigned>(splits)), dim3(kMergeThreads), 0, s, 1u, true, out, a.scratch,
-                     p.group, D, p.dtype);
+int launch_kv8(const Kv8Args& a, const PeerOut& out, int warps, cudaStream_t s) {
+  if (int st = launch_dependent(kv8_attention_kernel<C, D, SPLIT, SPARSE>, dim3(static_cast<unsigned>(warps)), dim3(32), ring_bytes<D>(), s, a, out))
+    return st;
+  const int items = a.tokens * a.kv_heads, lanes = a.group * D / 4;
+  auto merge = [&](auto kernel, int l) {
+    return launch_opts(kernel, dim3(static_cast<unsigned>(items), static_cast<unsigned>((lanes + l - 1) / l)), dim3(kMergeThreads), 0, s, 1u, true, a, out,
+                       D, warps);
+  };
+  if (items <= sm_count() || lanes <= 32) return merge(kv8_attention_merge_kernel<32>, 32);
+  return lanes <= 128 ? merge(kv8_attention_merge_kernel<128>, 128) : merge(kv8_attention_merge_kernel<256>, 256);
 }
 
 template <typename C, bool SPARSE>
-int dispatch_kv8(int64_t d, const Kv8Args& p, const PeerOut& out, int splits, cudaStream_t s) {
-  const bool split = p.dtype == XDK_F32;
+int dispatch_kv8(int64_t d, const Kv8Args& a, const PeerOut& out, int warps, cudaStream_t s) {
+  const bool split = a.dtype == XDK_F32;
   switch (d) {
-    case 64: return split ? launch_kv8<C, 64, true, SPARSE>(p, out, splits, s) : launch_kv8<C, 64, false, SPARSE>(p, out, splits, s);
-    case 128: return split ? launch_kv8<C, 128, true, SPARSE>(p, out, splits, s) : launch_kv8<C, 128, false, SPARSE>(p, out, splits, s);
-    case 256: return split ? launch_kv8<C, 256, true, SPARSE>(p, out, splits, s) : launch_kv8<C, 256, false, SPARSE>(p, out, splits, s);
+    case 64: return split ? launch_kv8<C, 64, true, SPARSE>(a, out, warps, s) : launch_kv8<C, 64, false, SPARSE>(a, out, warps, s);
+    case 128: return split ? launch_kv8<C, 128, true, SPARSE>(a, out, warps, s) : launch_kv8<C, 128, false, SPARSE>(a, out, warps, s);
+    case 256: return split ? launch_kv8<C, 256, true, SPARSE>(a, out, warps, s) : launch_kv8<C, 256, false, SPARSE>(a, out, warps, s);
     default: return XDK_ERR_LIMIT;
   }
 }
@@ -566,7 +670,7 @@ int dispatch_kv8(int64_t d, const Kv8Args& p, const PeerOut& out, int splits, cu
 int kv8_arguments(const void* q, const void* k_cache, const void* v_cache, const float* k_scale, const float* v_scale,
                   const int64_t* positions, const int64_t* page_table, const int64_t* sequence_ids, const xdk_peer_out* out_dst,
                   int64_t tokens, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t max_pages, int64_t page_size, int hnd,
-                  float scale, int dtype, int codes, unsigned flags, Kv8Args* p, PeerOut* out) {
+                  float scale, int dtype, int codes, unsigned flags, Kv8Args* a, PeerOut* out) {
   if (int st = make_out(out_dst, nullptr, 1, out)) return st;
   if (flags & ~XDK_DEPENDENT_LAUNCH) return XDK_ERR_ARG;
   if (!q || !k_cache || !v_cache || !k_scale || !v_scale || !positions || !page_table || !sequence_ids) return XDK_ERR_ARG;
@@ -575,43 +679,40 @@ int kv8_arguments(const void* q, const void* k_cache, const void* v_cache, const
   if (!aligned16(k_cache) || !aligned16(v_cache)) return XDK_ERR_ARG;
   if (dtype != XDK_F32 && dtype != XDK_BF16 && dtype != XDK_F16) return XDK_ERR_ARG;
   if (codes != XDK_KV8_INT8 && codes != XDK_KV8_E4M3) return XDK_ERR_ARG;
-  if (!kv8_head_dim(head_dim) || q_heads / kv_heads > kMaxGroup || tokens > 65535) return XDK_ERR_LIMIT;
+  if (!kv8_head_dim(head_dim) || q_heads / kv_heads > kMaxGroup || tokens > 65535 || tokens * kv_heads > (1 << 26)) return XDK_ERR_LIMIT;
   if (int st = kv8_limits(tokens, kv_heads, max_pages, page_size)) return st;
-  if (int st = require_sm100()) return st;
-  *p = {};
-  AttnArgs& a = p->at;
-  a.positions = positions, a.page_table = page_table, a.sequence_ids = sequence_ids;
-  a.max_pages = max_pages, a.page_size = page_size;
-  a.q_heads = static_cast<int>(q_heads), a.kv_heads = static_cast<int>(kv_heads);
-  a.hnd = hnd ? 1 : 0;
-  a.narrow = page_size * max_pages < (1LL << 31) ? 1 : 0;
-  a.scale = scale;
-  a.tokens = static_cast<int>(tokens);
-  a.scratch = nullptr;
-  p->q = q, p->k_cache = static_cast<const uint8_t*>(k_cache), p->v_cache = static_cast<const uint8_t*>(v_cache);
-  p->k_scale = k_scale, p->v_scale = v_scale;
-  p->group = static_cast<int>(q_heads / kv_heads), p->dtype = dtype;
+  *a = {};
+  a->q = q, a->k_cache = static_cast<const uint8_t*>(k_cache), a->v_cache = static_cast<const uint8_t*>(v_cache);
+  a->k_scale = k_scale, a->v_scale = v_scale;
+  a->positions = positions, a->page_table = page_table, a->sequence_ids = sequence_ids;
+  a->max_pages = max_pages, a->page_size = page_size;
+  a->tokens = static_cast<int>(tokens), a->q_heads = static_cast<int>(q_heads), a->kv_heads = static_cast<int>(kv_heads);
+  a->group = static_cast<int>(q_heads / kv_heads), a->dtype = dtype;
+  a->hnd = hnd ? 1 : 0;
+  a->narrow = page_size * max_pages < (1LL << 31) ? 1 : 0;
+  a->scale = scale;
+  a->tile = tile_of(head_dim);
   return XDK_OK;
 }
-// Splits of the items over the CTAs of a cluster: one wave of the SMs, no more than `tiles`, at most the portable cluster size.
-int cluster_splits(int64_t tokens, int64_t kv_heads, int64_t dim, int64_t tiles) {
-  int64_t splits = resident(dim) * sm_count() / (tokens * kv_heads);
-  if (splits > tiles) splits = tiles;
-  if (splits > kMaxSplits) splits = kMaxSplits;
-  return splits < 1 ? 1 : static_cast<int>(splits);
+size_t scratch_for(int64_t tokens, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t tiles) {
+  if (tokens < 1 || tokens > 65535 || kv_heads < 1 || kv_heads > 65535 || q_heads < kv_heads || q_heads % kv_heads != 0) return 0;
+  if (q_heads / kv_heads > kMaxGroup || !kv8_head_dim(head_dim) || tokens * kv_heads > (1 << 26)) return 0;
+  return partial_bytes(static_cast<size_t>(grid_for(tokens * kv_heads, head_dim, tiles)), static_cast<size_t>(tokens * kv_heads),
+                       static_cast<size_t>(q_heads / kv_heads * head_dim));
 }
 
 }  // namespace
+
 }  // namespace xdk
 
 extern "C" size_t xdk_kv8_decode_attention_scratch_bytes(int64_t tokens, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
                                                          int64_t context_hint) {
-  using namespace xdk;
-  if (tokens < 1 || q_heads < 1 || kv_heads < 1 || kv_heads > 65535 || q_heads % kv_heads != 0 || q_heads / kv_heads > kMaxGroup) return 0;
-  if (!kv8_head_dim(head_dim)) return 0;
-  if (context_hint <= 0 || context_hint > kMaxContextHint) context_hint = kMaxContextHint;
-  return static_cast<size_t>(kv8_even_grid(tokens, kv_heads, head_dim, context_hint)) *
-         partial_words(static_cast<size_t>(q_heads / kv_heads), static_cast<size_t>(head_dim)) * 4;
+  return xdk::scratch_for(tokens, q_heads, kv_heads, head_dim, xdk::hint_tiles(context_hint, head_dim));
+}
+extern "C" size_t xdk_kv8_sparse_attention_scratch_bytes(int64_t tokens, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
+                                                         int64_t page_size, int64_t n_pages) {
+  if (page_size < 1 || n_pages < 1 || page_size > xdk::kKV8MaxPage || n_pages > 2147483647LL / xdk::kKV8MaxPage) return 0;
+  return xdk::scratch_for(tokens, q_heads, kv_heads, head_dim, xdk::hint_tiles(n_pages * page_size, head_dim));
 }
 
 extern "C" int xdk_kv8_decode_attention(const void* q, const void* k_cache, const void* v_cache, const float* k_scale, const float* v_scale,
@@ -620,47 +721,44 @@ extern "C" int xdk_kv8_decode_attention(const void* q, const void* k_cache, cons
                                         int64_t max_pages_per_seq, int64_t page_size, int cache_is_hnd, float scale, int64_t context_hint,
                                         int dtype, int codes, void* scratch, size_t scratch_bytes, unsigned flags, void* stream) {
   using namespace xdk;
-  Kv8Args p;
+  Kv8Args a;
   PeerOut out;
   if (int st = kv8_arguments(q, k_cache, v_cache, k_scale, v_scale, positions, page_table, sequence_ids, out_dst, tokens, q_heads, kv_heads,
-                             head_dim, max_pages_per_seq, page_size, cache_is_hnd, scale, dtype, codes, flags, &p, &out))
+                             head_dim, max_pages_per_seq, page_size, cache_is_hnd, scale, dtype, codes, flags, &a, &out))
     return st;
+  if (!scratch || !aligned16(scratch) ||
+      scratch_bytes < xdk_kv8_decode_attention_scratch_bytes(tokens, q_heads, kv_heads, head_dim, context_hint))
+    return XDK_ERR_ARG;
+  if (int st = require_sm100()) return st;
   CallFlagsScope scope(flags);
-  // no bound from the caller: a row of the page table has one
-  const int64_t most = max_pages_per_seq * page_size;  // at most 2^41
-  if (context_hint <= 0) context_hint = most;
-  if (context_hint > kMaxContextHint) context_hint = kMaxContextHint;
-  int splits = 0;
-  if (scratch && aligned16(scratch)) {
-    const size_t need = xdk_kv8_decode_attention_scratch_bytes(tokens, q_heads, kv_heads, head_dim, context_hint);
-    if (need > 0 && scratch_bytes >= need) {
-      p.at.scratch = static_cast<float*>(scratch);
-      splits = kv8_even_grid(tokens, kv_heads, head_dim, context_hint);
-    }
-  }
-  if (!p.at.scratch) splits = cluster_splits(tokens, kv_heads, head_dim, (context_hint + kAttnThreads - 1) / kAttnThreads);
+  a.scratch = static_cast<float*>(scratch);
+  const int warps = grid_for(tokens * kv_heads, head_dim, hint_tiles(context_hint, head_dim));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return codes == XDK_KV8_INT8 ? dispatch_kv8<Int8Codes, false>(head_dim, p, out, splits, s)
-                               : dispatch_kv8<E4m3Codes, false>(head_dim, p, out, splits, s);
+  return codes == XDK_KV8_INT8 ? dispatch_kv8<Int8Codes, false>(head_dim, a, out, warps, s) : dispatch_kv8<E4m3Codes, false>(head_dim, a, out, warps, s);
 }
 
 extern "C" int xdk_kv8_sparse_attention(const void* q, const void* k_cache, const void* v_cache, const float* k_scale, const float* v_scale,
                                         const int32_t* pages, const int64_t* positions, const int64_t* page_table,
                                         const int64_t* sequence_ids, const xdk_peer_out* out_dst, int64_t tokens, int64_t q_heads,
                                         int64_t kv_heads, int64_t head_dim, int64_t max_pages_per_seq, int64_t page_size, int64_t n_pages,
-                                        int cache_is_hnd, float scale, int dtype, int codes, unsigned flags, void* stream) {
+                                        int cache_is_hnd, float scale, int dtype, int codes, void* scratch, size_t scratch_bytes,
+                                        unsigned flags, void* stream) {
   using namespace xdk;
-  Kv8Args p;
+  Kv8Args a;
   PeerOut out;
   if (!pages || n_pages < 1) return XDK_ERR_ARG;
   if (n_pages > 2147483647LL / kKV8MaxPage) return XDK_ERR_LIMIT;
   if (int st = kv8_arguments(q, k_cache, v_cache, k_scale, v_scale, positions, page_table, sequence_ids, out_dst, tokens, q_heads, kv_heads,
-                             head_dim, max_pages_per_seq, page_size, cache_is_hnd, scale, dtype, codes, flags, &p, &out))
+                             head_dim, max_pages_per_seq, page_size, cache_is_hnd, scale, dtype, codes, flags, &a, &out))
     return st;
+  if (!scratch || !aligned16(scratch) ||
+      scratch_bytes < xdk_kv8_sparse_attention_scratch_bytes(tokens, q_heads, kv_heads, head_dim, page_size, n_pages))
+    return XDK_ERR_ARG;
+  if (int st = require_sm100()) return st;
   CallFlagsScope scope(flags);
-  p.pages = pages, p.n_pages = static_cast<int>(n_pages);
-  const int splits = cluster_splits(tokens, kv_heads, head_dim, (n_pages * page_size + kAttnThreads - 1) / kAttnThreads);
+  a.pages = pages, a.n_pages = static_cast<int>(n_pages);
+  a.scratch = static_cast<float*>(scratch);
+  const int warps = grid_for(tokens * kv_heads, head_dim, hint_tiles(n_pages * page_size, head_dim));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return codes == XDK_KV8_INT8 ? dispatch_kv8<Int8Codes, true>(head_dim, p, out, splits, s)
-                               : dispatch_kv8<E4m3Codes, true>(head_dim, p, out, splits, s);
+  return codes == XDK_KV8_INT8 ? dispatch_kv8<Int8Codes, true>(head_dim, a, out, warps, s) : dispatch_kv8<E4m3Codes, true>(head_dim, a, out, warps, s);
 }

@@ -230,12 +230,12 @@ def paged_kv8_decode_attention(q, cache: PagedKV8Cache, positions, page_table, s
             hint = page_table.shape[1] * cache.page_size
         hint = min(hint, 2 ** 62)
         need = lib.xdk_kv8_decode_attention_scratch_bytes(tokens, q_heads, cache.kv_heads, cache.head_dim, hint)
-        scratch = torch.empty(need, device=q.device, dtype=torch.uint8) if need else None
+        scratch = torch.empty(need, device=q.device, dtype=torch.uint8)
         status = lib.xdk_kv8_decode_attention(
             q.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), positions.data_ptr(),
             page_table.data_ptr(), sequence_ids.data_ptr(), ctypes.byref(dst), tokens, q_heads, cache.kv_heads, cache.head_dim,
             page_table.shape[1], cache.page_size, int(cache.hnd), scale, hint, _native.dtype_code(q.dtype), _CODES[cache.k.dtype],
-            scratch.data_ptr() if need else None, need, _flags(dependent_launch), _native.stream_ptr(q.device))
+            scratch.data_ptr(), need, _flags(dependent_launch), _native.stream_ptr(q.device))
     _native.check(status, "xdk_kv8_decode_attention")
     return out
 
@@ -280,11 +280,14 @@ def paged_kv8_sparse_attention(q, cache: PagedKV8Cache, pages, positions, page_t
     _need(pages.dim() == 3 and tuple(pages.shape[:2]) == (tokens, cache.kv_heads) and pages.shape[2] > 0, "pages must be [tokens, kv_heads, n]")
     _need(pages.shape[2] <= (2 ** 31 - 1) // MAX_PAGE_SIZE, "too many pages per token")
     with torch.cuda.device(q.device):
+        lib = _native.lib()
         out, dst = _destination(q, peer_out)
-        status = _native.lib().xdk_kv8_sparse_attention(
+        need = lib.xdk_kv8_sparse_attention_scratch_bytes(tokens, q_heads, cache.kv_heads, cache.head_dim, cache.page_size, pages.shape[2])
+        scratch = torch.empty(need, device=q.device, dtype=torch.uint8)
+        status = lib.xdk_kv8_sparse_attention(
             q.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), pages.data_ptr(),
             positions.data_ptr(), page_table.data_ptr(), sequence_ids.data_ptr(), ctypes.byref(dst), tokens, q_heads, cache.kv_heads,
             cache.head_dim, page_table.shape[1], cache.page_size, pages.shape[2], int(cache.hnd), scale, _native.dtype_code(q.dtype),
-            _CODES[cache.k.dtype], _flags(dependent_launch), _native.stream_ptr(q.device))
+            _CODES[cache.k.dtype], scratch.data_ptr(), need, _flags(dependent_launch), _native.stream_ptr(q.device))
     _native.check(status, "xdk_kv8_sparse_attention")
     return out

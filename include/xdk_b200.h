@@ -320,14 +320,16 @@ XDK_API int xdk_swiglu_peer(const void* upgate, const xdk_peer_out* out_dst, int
  *   q_out is contiguous; k_mean may be NULL (no means).  scratch: xdk_kv8_append_scratch_bytes(tokens) bytes (0 for
  *   small batches), content undefined, not shared by calls that may overlap on the GPU; one memset and two launches then, one launch else.
  * xdk_kv8_decode_attention: xdk_paged_decode_attention_ws for this cache: any q_heads / kv_heads up to 8; softmax and sums in FP32; a context
- *   of no positions (positions[t] < 0) gives 0.
+ *   of no positions (positions[t] < 0) gives 0.  Two launches.  scratch: xdk_kv8_decode_attention_scratch_bytes(..., the same context_hint)
+ *   bytes, content undefined, not shared by calls that may overlap on the GPU.
  * xdk_kv8_select_pages: per token and KV head the last page of the context and the top_pages - 1 others with the best scores,
  *   score = max over the heads of the group of (unit * (qc . k_mean)) * k_scale, qc = round(q / unit), unit = max |q| * (1 / 127), the
  *   lowest page first among equals.  pages: int32 [tokens, kv_heads, top_pages], logical pages, ascending, -1 behind the last one; all -1 for a
  *   position < 0.  k_mean has to hold the means of all pages in front of the last one (the append writes them as blocks fill up).
  *   q_heads / kv_heads <= 8; at most 51200 pages per sequence (XDK_ERR_LIMIT).
  * xdk_kv8_sparse_attention: the attention over the positions of the listed pages, [tokens, kv_heads, n_pages], ascending; an entry that is
- *   negative, not above the one before, or behind the context adds nothing.  One launch, no scratch.
+ *   negative, not above the one before, or behind the context adds nothing.  Two launches; scratch as above, of
+ *   xdk_kv8_sparse_attention_scratch_bytes.
  */
 typedef enum xdk_kv8_codes { XDK_KV8_INT8 = 0, XDK_KV8_E4M3 = 1 } xdk_kv8_codes;
 XDK_API size_t xdk_kv8_append_scratch_bytes(int64_t tokens);
@@ -344,6 +346,8 @@ XDK_API int xdk_kv8_decode_attention(const void* q, const void* k_cache, const v
                              const xdk_peer_out* out_dst, int64_t tokens, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
                              int64_t max_pages_per_seq, int64_t page_size, int cache_is_hnd, float scale, int64_t context_hint,
                              int dtype, int codes, void* scratch, size_t scratch_bytes, unsigned flags, void* stream);
+XDK_API size_t xdk_kv8_sparse_attention_scratch_bytes(int64_t tokens, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
+                                              int64_t page_size, int64_t n_pages);
 XDK_API int xdk_kv8_select_pages(const void* q, const int8_t* k_mean, const float* k_scale, const int64_t* positions,
                          const int64_t* page_table, const int64_t* sequence_ids, int32_t* pages, int64_t tokens, int64_t q_heads,
                          int64_t kv_heads, int64_t head_dim, int64_t max_pages_per_seq, int64_t page_size, int64_t top_pages,
@@ -352,7 +356,8 @@ XDK_API int xdk_kv8_sparse_attention(const void* q, const void* k_cache, const v
                              const int32_t* pages, const int64_t* positions, const int64_t* page_table,
                              const int64_t* sequence_ids, const xdk_peer_out* out_dst, int64_t tokens, int64_t q_heads,
                              int64_t kv_heads, int64_t head_dim, int64_t max_pages_per_seq, int64_t page_size, int64_t n_pages,
-                             int cache_is_hnd, float scale, int dtype, int codes, unsigned flags, void* stream);
+                             int cache_is_hnd, float scale, int dtype, int codes, void* scratch, size_t scratch_bytes,
+                             unsigned flags, void* stream);
 
 /*
  * Symmetric INT4 quantisation on the device, into the format xdk_w4a16 reads: weight [n, k] row-major of

@@ -80,13 +80,15 @@ def append(q, k, v, cos, sin, positions, page_table, sequence_ids, cache, *, rop
 
 
 def attention(q, cache, positions, page_table, sequence_ids, *, scale=None, pages=None):
-    """(result, bound, score, least): the result in 64 bits; for every element of it sum_j p_j |v_j|; for every head the largest
-    scale * sum_d |q_d k_d| of a position; for every element max_j(p_j vs_j) * sum_j |code_j|, vs the scales of V.
+    """A dict: `result` in 64 bits; for every element of it `bound`, sum_j p_j |v_j|, and `least`, max_j(p_j vs_j) * sum_j |code_j|, vs
+    the scales of V; for every head `score`, the largest scale * sum_d |q_d k_d| of a position, `offset`, the largest
+    scale * ks * max(|sum of q_d over d >= 16 c|, 2 |q_d|), and `flat`, sum_j p_j vs_j.
     `pages` [tokens, kv_heads, n]: only these."""
     page_size, heads, dim = cache["k"].shape[1:]
     scale = dim ** -0.5 if scale is None else scale
     out = torch.zeros(q.shape, dtype=torch.float64)
-    bound, least, score = torch.zeros_like(out), torch.zeros_like(out), torch.zeros(q.shape[:2], dtype=torch.float64)
+    bound, least = torch.zeros_like(out), torch.zeros_like(out)
+    score, offset, flat = (torch.zeros(q.shape[:2], dtype=torch.float64) for _ in range(3))
     group = q.shape[1] // heads
     for t, pos in enumerate(positions.tolist()):
         for h in range(heads):
@@ -108,8 +110,11 @@ def attention(q, cache, positions, page_table, sequence_ids, *, scale=None, page
             p = torch.softmax(x @ k.T * scale, dim=-1)
             out[t, mine], bound[t, mine] = p @ v, p @ v.abs()
             least[t, mine] = (p * cache["v_scale"][at, h].double().abs()).amax(-1, keepdim=True) * cache["v"][at, off, h].double().abs().sum(0)
+            ks, vs = cache["k_scale"][at, h].double().abs(), cache["v_scale"][at, h].double()
+            ends = x.unflatten(-1, (dim // 16, 16)).sum(-1).flip(-1).cumsum(-1).abs().amax(-1).maximum(2 * x.abs().amax(-1))
+            offset[t, mine], flat[t, mine] = ends * ks.amax() * abs(scale), p @ vs
             score[t, mine] = (x.abs() @ k.abs().T * abs(scale)).amax(-1)
-    return out, bound, score, least
+    return dict(result=out, bound=bound, least=least, score=score, offset=offset, flat=flat)
 
 
 def select(q, cache, positions, page_table, sequence_ids, *, top_pages):

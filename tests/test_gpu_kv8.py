@@ -170,16 +170,20 @@ def test_append_takes_slices_of_a_fused_projection_and_wide_tables():
 def _close(got, exact, dtype, dim):
     """Half a step of the output type, and sum_j p_j |v_j| times what the weights are off by.  16-bit q: it is exact, a weight is rounded
     to FP16 once (2^-11 of it).  FP32 q: two FP16 numbers leave 2^-21 of a weight and of a product of the scores.  Either way FP32 sums:
-    a score is off by at most 2^-22 of sum |q_d k_d| per matrix product of its chain (truncation; 2 dim / 16 of them, and
-    its scaling), a weight by twice that (exp, and the sum it is divided by), and the accumulators by 2^-18.  Weights are
-    taken relative to the largest, times 2^14, so that a step of the smallest FP16 numbers, 2^-24, is 2^-38 of it: a code is off by half of
-    that, wherever the largest weight meets codes of 0 and nothing else is left to see."""
-    want, bound, score, least = exact
-    chain = 2 * dim // 16 + 4
-    weight = 2.0 ** (-21 if dtype == F32 else -11) + 2.0 ** -18 + 2 * score[..., None] * (chain * 2.0 ** -22 + 2.0 ** -21)
+    a score is off by at most 2^-22 of sum |q_d k_d| per matrix product of its chain (truncation; 2 dim / 16 of them, and its scaling), a
+    weight by twice that (exp, and the sum it is divided by), and the accumulators by 2^-18.  Weights are taken relative to the largest,
+    times 2^14, so that a step of the smallest FP16 numbers, 2^-24, is 2^-38 of it: a code is off by half of that, wherever the largest
+    weight meets codes of 0 and nothing else is left to see.  int8 codes under 16-bit q enter as code + 128: a matrix product
+    cuts its 16 terms and its sum at 2^-24 of the largest of them, which is up to 128 * |the sum of q_d behind it| or 256 * |q_d| (17 * 2^-24 < 2^-19 of
+    that, dim / 16 products to a score), or 256 * the weights (two products, and their own sum rounded 8 times: 2^-18 of 128 * the sum)."""
+    bound, score = exact["bound"], exact["score"]
+    chain, lift = 2 * dim // 16 + 4, 0.0 if dtype == F32 else 128.0
+    lost = 2 * (score * (chain * 2.0 ** -22 + 2.0 ** -21) + lift * exact["offset"] * dim / 16 * 2.0 ** -19)
+    weight = 2.0 ** (-21 if dtype == F32 else -11) + 2.0 ** -18 + lost[..., None]
     info = torch.finfo(dtype)  # half a step of a subnormal result is that of the smallest normal one
-    limit = bound * weight * 1.01 + least * 2.0 ** -39 + torch.clamp(want.abs(), min=info.smallest_normal) * info.eps / 2
-    finite, far = bool(torch.isfinite(got).all()), float(((got.double().cpu() - want).abs() / limit).max())
+    limit = bound * weight * 1.01 + exact["least"] * 2.0 ** -39 + lift * exact["flat"][..., None] * 2.0 ** -18
+    limit = limit + torch.clamp(exact["result"].abs(), min=info.smallest_normal) * info.eps / 2
+    finite, far = bool(torch.isfinite(got).all()), float(((got.double().cpu() - exact["result"]).abs() / limit).max())
     assert finite and far <= 1.0
 
 
@@ -231,8 +235,8 @@ def test_attention_over_scales_of_any_size(codes, dtype):
     q = q.to(dtype)
     exact = oracle.attention(q, cache, pos, table, seq)
     if dtype == F16:  # results beyond the type are infinite
-        keep = exact[0].abs().amax(-1, keepdim=True) < 6e4
-        exact = [x * keep if x.dim() == 3 else x for x in exact]
+        keep = exact["result"].abs().amax(-1, keepdim=True) < 6e4
+        exact = {name: x * (keep if x.dim() == 3 else keep[..., 0]) for name, x in exact.items()}
     got = paged_kv8_decode_attention(q.cuda(), _on_gpu(cache, "NHD"), *(t.cuda() for t in (pos, table, seq)))
     if dtype == F16:
         got = torch.where(keep.cuda(), got, torch.zeros_like(got))

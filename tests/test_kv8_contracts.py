@@ -76,12 +76,12 @@ def test_c_entry_points_check_sizes_before_they_touch_a_gpu():
     def attend(q=p, k=p, codes=0, dtype=0, scale=1.0, flags=0, dst=out, **kw):
         s = {**good, **kw}
         return lib.xdk_kv8_decode_attention(q, k, p, p, p, p, p, p, dst, s["tokens"], s["hq"], s["hkv"], s["dim"], s["width"], s["page"], 0, scale, 0,
-                                            dtype, codes, None, 0, flags, None)
+                                            dtype, codes, kw.get("scratch"), kw.get("nbytes", 0), flags, None)
 
     def sparse(n=1, pages=p, **kw):
         s = {**good, **kw}
         return lib.xdk_kv8_sparse_attention(p, p, p, p, p, pages, p, p, p, out, s["tokens"], s["hq"], s["hkv"], s["dim"], s["width"], s["page"], n, 0, 1.0,
-                                            0, 0, 0, None)
+                                            0, 0, kw.get("scratch"), kw.get("nbytes", 0), 0, None)
 
     def select(top=1, mean=p, **kw):
         s = {**good, **kw}
@@ -94,14 +94,15 @@ def test_c_entry_points_check_sizes_before_they_touch_a_gpu():
 
     wrong, limit = -1, -4
     for kw in (dict(q=None), dict(k=None), dict(k=p + 8), dict(codes=2), dict(codes=-1), dict(dtype=3), dict(scale=float("nan")),
-               dict(scale=float("inf")), dict(flags=1), dict(dst=None), dict(tokens=0), dict(hq=3), dict(page=0), dict(width=0), dict(hq=8)):
+               dict(scale=float("inf")), dict(flags=1), dict(dst=None), dict(tokens=0), dict(hq=3), dict(page=0), dict(width=0), dict(hq=8),
+               dict(), dict(scratch=p, nbytes=64), dict(scratch=p + 8, nbytes=1 << 40)):
         assert attend(**kw) == wrong, kw
     for kw in (dict(tokens=65536), dict(dim=32), dict(page=1025), dict(width=1 << 31)):
         assert attend(**kw) == limit, kw
     dst.ld = 18 * 64
     assert attend(hq=18) == limit  # nine heads to a group
     dst.ld = 4 * 64
-    assert sparse(n=0) == wrong and sparse(pages=None) == wrong and sparse(n=1 << 22) == limit
+    assert sparse() == wrong and sparse(scratch=p, nbytes=64) == wrong and sparse(n=0) == wrong and sparse(pages=None) == wrong and sparse(n=1 << 22) == limit
     assert select(top=0) == wrong and select(mean=None) == wrong and select(mean=p + 4) == wrong and select(width=51201) == limit and select(hq=18) == limit
     for kw in (dict(cache=None), dict(cache=p + 1), dict(rope=3), dict(rope=66), dict(rope=0), dict(cw=31), dict(qs=255), dict(codes=2),
                dict(dtype=7), dict(flags=1), dict(tokens=129), dict(tokens=129, scratch=p, nbytes=64), dict(tokens=-1)):
@@ -109,8 +110,10 @@ def test_c_entry_points_check_sizes_before_they_touch_a_gpu():
     for kw in (dict(dim=192, qs=768), dict(page=2000), dict(tokens=(1 << 26) + 1)):
         assert append(**kw) in (limit, wrong), kw
     assert lib.xdk_kv8_append_scratch_bytes(128) == 0 and lib.xdk_kv8_append_scratch_bytes(129) >= 512 * 20
-    assert lib.xdk_kv8_decode_attention_scratch_bytes(1, 4, 2, 64, 1024) == 0  # short: one launch
-    assert lib.xdk_kv8_decode_attention_scratch_bytes(1, 4, 2, 64, 8192) > 0 and lib.xdk_kv8_decode_attention_scratch_bytes(1, 18, 2, 64, 8192) == 0
+    size = lib.xdk_kv8_decode_attention_scratch_bytes
+    assert 0 < size(1, 4, 2, 64, 1024) < size(1, 4, 2, 64, 8192) <= size(1, 4, 2, 64, 0) == size(1, 4, 2, 64, 1 << 62)
+    assert size(1, 18, 2, 64, 8192) == size(0, 4, 2, 64, 64) == size(1, 4, 2, 96, 64) == size(1, 4, 3, 64, 64) == 0
+    assert lib.xdk_kv8_sparse_attention_scratch_bytes(1, 4, 2, 64, 16, 8) > 0 == lib.xdk_kv8_sparse_attention_scratch_bytes(1, 4, 2, 64, 16, 0)
 
 
 def _inputs():
