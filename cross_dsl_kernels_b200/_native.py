@@ -49,7 +49,7 @@ SIGNATURES = {
     "xdk_paged_decode_attention_scratch_bytes": (ctypes.c_size_t, [_i64] * 5 + [_int]),
     "xdk_paged_decode_attention_ws": (_int, [_p] * 7 + [_i64] * 6 + [_int, ctypes.c_float, _i64, _int, _p, ctypes.c_size_t, _uint, _p]),
     "xdk_swiglu_peer": (_int, [_p, _p, _i64, _i64, _i64, _int, _uint, _p]),
-    "xdk_kv8_append_scratch_bytes": (ctypes.c_size_t, [_i64]),
+    "xdk_kv8_append_scratch_bytes": (ctypes.c_size_t, [_i64] * 2),
     "xdk_kv8_append": (_int, [_p] * 14 + [_i64] * 11 + [_int] * 4 + [_p, ctypes.c_size_t, _uint, _p]),
     "xdk_kv8_decode_attention_scratch_bytes": (ctypes.c_size_t, [_i64] * 5),
     "xdk_kv8_decode_attention": (_int, [_p] * 9 + [_i64] * 6 + [_int, ctypes.c_float, _i64, _int, _int, _p, ctypes.c_size_t, _uint, _p]),

@@ -383,7 +383,7 @@ PyObject* kv8_append(PyObject*, PyObject* const* arg, Py_ssize_t n) {
     Unlocked unlocked;
     c10::cuda::CUDAGuard guard(c.q->device());
     out = at::empty(c.q->sizes(), c.q->options());
-    const size_t need = xdk_kv8_append_scratch_bytes(c.tokens);
+    const size_t need = xdk_kv8_append_scratch_bytes(c.tokens, c.hkv);
     at::Tensor scratch;
     if (need) scratch = at::empty({static_cast<int64_t>(need)}, c.q->options().dtype(at::kByte));
     const bool many = c.tokens > 1;

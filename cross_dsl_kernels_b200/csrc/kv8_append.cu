@@ -10,12 +10,15 @@
 //     scale * 448 / 127 (e4m3)
 //   Every step is a correctly rounded FP32 operation or a sum of whole numbers: the bytes are defined, whatever the order.
 //
-// One CTA owns a block of K and V: it finds the rows from the batch's index vectors, so tokens may come in any order, several for
-// a page or for a slot.  Up to kSmallBatch tokens every CTA looks all of them up (one launch; the first token of a page does its
-// work); longer batches are grouped by page in a table in scratch while Q is rotated, and a second launch walks the groups.
+// A block's rows come from the batch's index vectors, so tokens may come in any order, several for a page or for a slot.  Up to
+// kSmallBatch tokens: one launch, every CTA looks all of them up, and the first token of a page does its work, a warp to a block.  Longer
+// batches: the first launch enters the tokens by page into a table in scratch, rotates Q, and leaves the largest value of every row of K and
+// V; the second one walks the table, and can write a row at once.  (Blocks that first read their rows for the largest value and then write them, in
+// one kernel: a CTA to a block 46 us for 4096 tokens, a warp to a block 49, 36 of it in its chain of loads.)
+// A lane holds two vectors of eight dims of a row, rotation partners where there are some, and so reads every value and angle once.
 //
 // Bound: a decode batch by its chain of dependent loads (position, sequence, page, then the block's scale), a prefill chunk by
-// HBM (values read once, codes written once).
+// HBM (values read once, codes written once; the second launch finds them in L2) and its two launches.
 #include <math.h>
 
 #include "kv8.cuh"
@@ -40,7 +43,8 @@ struct AppendArgs {
   float mean_unit;
 };
 
-// Where the tokens of a long batch go, by physical page: an open hash table of `slots` entries, all bytes 0xff before the call.
+// Where the tokens of a long batch go, by physical page: an open hash table of `slots` entries; what stands up to `count` is
+// filled with 0xff before the first launch.
 struct Groups {
   unsigned long long* page;  // [slots], ~0: free
   unsigned* first;           // [slots] first and last token of the page
@@ -48,6 +52,8 @@ struct Groups {
   int* list;                 // [slots] the entries in use, in any order
   int* slot_of;              // [tokens] entry of a token's page, -1: no page
   int* count;                // entries in use - 1
+  unsigned* tops;            // [tokens, 2 * kv_heads] the bits of the largest |value| of a row of K, then of V
+  uint16_t* row_of;          // [tokens] row in the page
   unsigned mask;             // slots - 1
 };
 inline int64_t group_slots(int64_t tokens) {
@@ -55,21 +61,26 @@ inline int64_t group_slots(int64_t tokens) {
   while (s < 2 * tokens) s <<= 1;
   return s;
 }
-inline size_t group_bytes(int64_t tokens) { return static_cast<size_t>(group_slots(tokens)) * 20 + static_cast<size_t>(tokens + 1) * 4; }
-inline Groups groups_at(void* scratch, int64_t tokens) {
+inline size_t cleared_bytes(int64_t tokens) { return static_cast<size_t>(group_slots(tokens)) * 20 + 4; }
+inline size_t group_bytes(int64_t tokens, int64_t kv_heads) {
+  return cleared_bytes(tokens) + static_cast<size_t>(tokens) * static_cast<size_t>(4 + 2 + 8 * kv_heads);
+}
+inline Groups groups_at(void* scratch, int64_t tokens, int64_t kv_heads) {
   const int64_t s = group_slots(tokens);
   Groups g;
   g.page = static_cast<unsigned long long*>(scratch);
   g.first = reinterpret_cast<unsigned*>(g.page + s);
   g.last = reinterpret_cast<int*>(g.first + s);
   g.list = g.last + s;
-  g.slot_of = g.list + s;
-  g.count = g.slot_of + tokens;
+  g.count = g.list + s;
+  g.slot_of = g.count + 1;
+  g.tops = reinterpret_cast<unsigned*>(g.slot_of + tokens);
+  g.row_of = reinterpret_cast<uint16_t*>(g.tops + tokens * 2 * kv_heads);
   g.mask = static_cast<unsigned>(s - 1);
   return g;
 }
 
-template <typename T, bool VEC> __device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
+template <typename T, bool VEC> __device__ __forceinline__ void load8(const T* p, float* x) {
   if constexpr (VEC) {
     constexpr int E = Elem<T>::kPerVec;
 #pragma unroll
@@ -84,210 +95,266 @@ template <typename T, bool VEC> __device__ __forceinline__ void load8(const T* p
     for (int e = 0; e < 8; ++e) x[e] = Elem<T>::to_f32(p[e]);
   }
 }
-template <bool VEC> __device__ __forceinline__ void load_angles(const float* p, float* x, int n) {  // n: 4 or 8, 16-byte aligned if VEC
+// The two vectors of eight dims that thread t of a row's D / 16 holds: rotation partners, where these are whole vectors, or two next
+// to each other.
+template <bool VEC> __device__ __forceinline__ void dims_of(const AppendArgs& a, int t, int& d0, int& d1) {
+  const int pairs = !VEC || a.interleaved ? 0 : a.rope_dim / 16;
+  if (t < pairs) d0 = t * 8, d1 = d0 + a.rope_dim / 2;
+  else d0 = pairs * 16 + (t - pairs) * 16, d1 = d0 + 8;
+}
+// Angles of the pairs in vectors d0, d1: eight of a non-interleaved pair of vectors, four of each of interleaved ones.
+__device__ __forceinline__ void angles_of(const AppendArgs& a, int d0, int d1, int64_t pos, float (&c)[8], float (&s)[8]) {
+  const float *crow = a.cos + pos * a.cos_width, *srow = a.sin + pos * a.cos_width;
+  auto load = [](const float* p, float* x) {
+    const float4 f = __ldg(reinterpret_cast<const float4*>(p));
+    x[0] = f.x, x[1] = f.y, x[2] = f.z, x[3] = f.w;
+  };
+  const bool first = d0 < a.rope_dim, second = d1 < a.rope_dim;
+  const int at0 = a.interleaved ? d0 / 2 : d0, at1 = a.interleaved ? d1 / 2 : d0 + 4;
+  if (first) load(crow + at0, c), load(srow + at0, s);
+  if (second) load(crow + at1, c + 4), load(srow + at1, s + 4);
+}
+// Turns x (at dims d0 .. and d1 ..) by the angles; separately rounded products and sums.
+__device__ __forceinline__ void turn(const AppendArgs& a, int d0, int d1, const float (&c)[8], const float (&s)[8], float (&x)[16]) {
+  auto pair = [](float& lo, float& hi, float cv, float sv) {
+    const float l = lo, h = hi;
+    lo = __fsub_rn(__fmul_rn(l, cv), __fmul_rn(h, sv));
+    hi = __fadd_rn(__fmul_rn(l, sv), __fmul_rn(h, cv));
+  };
+  if (a.interleaved) {
+    if (d0 < a.rope_dim)
 #pragma unroll
-  for (int i = 0; i < 8; i += 4) {
-    if (i >= n) break;
-    if constexpr (VEC) {
-      const float4 f = __ldg(reinterpret_cast<const float4*>(p + i));
-      x[i] = f.x, x[i + 1] = f.y, x[i + 2] = f.z, x[i + 3] = f.w;
-    } else {
+      for (int e = 0; e < 4; ++e) pair(x[2 * e], x[2 * e + 1], c[e], s[e]);
+    if (d1 < a.rope_dim)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[i + e] = __ldg(p + i + e);
-    }
+      for (int e = 0; e < 4; ++e) pair(x[8 + 2 * e], x[9 + 2 * e], c[4 + e], s[4 + e]);
+  } else if (d0 < a.rope_dim) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) pair(x[e], x[8 + e], c[e], s[e]);
   }
 }
-
-// Dims d0 .. d0 + 7 of a head, rotated.  VEC: whole vectors are rotated or not, and partners and angles are 16-byte vectors too.
-template <typename T, bool VEC>
-__device__ __forceinline__ void rotated8(const AppendArgs& a, const T* head, int d0, int64_t pos, float (&x)[8]) {
-  load8<T, VEC>(head + d0, x);
+// Any rotation width and any alignment: dim by dim.
+template <typename T>
+__device__ __forceinline__ void rotated_scalar(const AppendArgs& a, const T* head, int d0, int64_t pos, float* x) {
   const float *crow = a.cos + pos * a.cos_width, *srow = a.sin + pos * a.cos_width;
   const int half = a.rope_dim / 2;
+  load8<T, false>(head + d0, x);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const int d = d0 + e;
+    if (d >= a.rope_dim) break;
+    const bool upper = a.interleaved ? (d & 1) != 0 : d >= half;
+    const int at = a.interleaved ? d >> 1 : (upper ? d - half : d);
+    const float p = Elem<T>::to_f32(head[a.interleaved ? d ^ 1 : (upper ? at : d + half)]);
+    const float c = __ldg(crow + at), s = __ldg(srow + at);
+    x[e] = upper ? __fadd_rn(__fmul_rn(p, s), __fmul_rn(x[e], c)) : __fsub_rn(__fmul_rn(x[e], c), __fmul_rn(p, s));
+  }
+}
+template <typename T, bool VEC>
+__device__ __forceinline__ void rotated16(const AppendArgs& a, const T* head, int d0, int d1, int64_t pos, float (&x)[16]) {
   if constexpr (VEC) {
-    if (d0 >= a.rope_dim) return;
     float c[8], s[8];
-    if (a.interleaved) {
-      load_angles<true>(crow + d0 / 2, c, 4), load_angles<true>(srow + d0 / 2, s, 4);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float lo = x[2 * e], hi = x[2 * e + 1];
-        x[2 * e] = __fsub_rn(__fmul_rn(lo, c[e]), __fmul_rn(hi, s[e]));
-        x[2 * e + 1] = __fadd_rn(__fmul_rn(lo, s[e]), __fmul_rn(hi, c[e]));
-      }
-      return;
-    }
-    const bool upper = d0 >= half;
-    const int at = upper ? d0 - half : d0;
-    float p[8];
-    load8<T, true>(head + (upper ? at : d0 + half), p);
-    load_angles<true>(crow + at, c, 8), load_angles<true>(srow + at, s, 8);
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      x[e] = upper ? __fadd_rn(__fmul_rn(p[e], s[e]), __fmul_rn(x[e], c[e])) : __fsub_rn(__fmul_rn(x[e], c[e]), __fmul_rn(p[e], s[e]));
+    load8<T, true>(head + d0, x), load8<T, true>(head + d1, x + 8);
+    angles_of(a, d0, d1, pos, c, s);
+    turn(a, d0, d1, c, s, x);
   } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int d = d0 + e;
-      if (d >= a.rope_dim) break;
-      const bool upper = a.interleaved ? (d & 1) != 0 : d >= half;
-      const int at = a.interleaved ? d >> 1 : (upper ? d - half : d);
-      const float p = Elem<T>::to_f32(head[a.interleaved ? d ^ 1 : (upper ? at : d + half)]);
-      const float c = __ldg(crow + at), s = __ldg(srow + at);
-      x[e] = upper ? __fadd_rn(__fmul_rn(p, s), __fmul_rn(x[e], c)) : __fsub_rn(__fmul_rn(x[e], c), __fmul_rn(p, s));
-    }
+    rotated_scalar(a, head, d0, pos, x), rotated_scalar(a, head, d1, pos, x + 8);
   }
 }
 
-// Eight dims of one Q head per thread; unit: of the token's q_heads * D / 8.  A token without a position gets zeros.
-template <typename T, int D, bool VEC>
-__device__ __forceinline__ void rotate_q(const AppendArgs& a, int token, int unit) {
-  if (unit >= a.q_heads * (D / 8)) return;
-  const int head = unit / (D / 8), d0 = (unit - head * (D / 8)) * 8;
-  const int64_t pos = a.positions[token];
-  float x[8] = {};
-  if (pos >= 0) rotated8<T, VEC>(a, static_cast<const T*>(a.q) + token * a.q_stride + head * D, d0, pos, x);
-  T* dst = static_cast<T*>(a.q_out) + (static_cast<int64_t>(token) * a.q_heads + head) * D + d0;  // torch's own, or 16-byte aligned
-  constexpr int E = Elem<T>::kPerVec;
-#pragma unroll
-  for (int i = 0; i < 8 / E; ++i) {
-    float f[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) f[e] = x[i * E + e];
-    *reinterpret_cast<U4*>(dst + i * E) = pack16<T>(f);
-  }
+// A unit: a thread has the same 16 dims of a few heads of a token, of Q, of K or of V, so the angles are loaded once for them.  Q is
+// rotated and written (a token without a position gets zeros); of K, rotated, and of V the largest values of the rows are left in `tops`.
+template <typename T> constexpr int kHeadsOf = sizeof(T) == 4 ? 2 : 4;
+template <typename T, int D> __host__ __device__ constexpr int units_of(int heads) {  // threads of a token
+  return (heads + (sizeof(T) == 4 ? 2 : 4) - 1) / (sizeof(T) == 4 ? 2 : 4) * (D / 16);
 }
-
-struct BlockShared {
-  int token_of[kKV8MaxPage];  // row -> token, -1: not written by this call
-  unsigned top_k[kThreads / 32], top_v[kThreads / 32];
-  int sums[256];
-};
-
-__device__ __forceinline__ unsigned largest8(unsigned top, const float (&x)[8]) {  // of the bits of |x|: NaN over infinity over numbers
+__device__ __forceinline__ unsigned largest(const float (&x)[16]) {  // the bits of the largest |value|: NaN over infinity over numbers
+  unsigned top = 0;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
+  for (int e = 0; e < 16; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
   return top;
 }
-// The scale behind the call from the one before and the largest value: NaN for anything that is not a finite number.
+template <int D> __device__ __forceinline__ unsigned row_max(unsigned top) {  // over the D / 16 lanes of a row
+#pragma unroll
+  for (int sh = 1; sh < D / 16; sh <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, sh));
+  return top;
+}
+template <typename T, int D, bool VEC>
+__device__ __forceinline__ void rotate_q(const AppendArgs& a, int token, int rest) {  // rest: unit of the token's heads of Q
+  constexpr int kHeads = kHeadsOf<T>, E = Elem<T>::kPerVec;
+  const int head0 = rest / (D / 16) * kHeads, heads = a.q_heads - head0 < kHeads ? a.q_heads - head0 : kHeads;
+  int d0, d1;
+  dims_of<VEC>(a, rest % (D / 16), d0, d1);
+  const int64_t pos = a.positions[token];
+  const T* src = static_cast<const T*>(a.q) + token * a.q_stride + head0 * D;
+  T* dst = static_cast<T*>(a.q_out) + (static_cast<int64_t>(token) * a.q_heads + head0) * D;  // 16-byte aligned
+  float c[8], s[8];
+  if (VEC && pos >= 0) angles_of(a, d0, d1, pos, c, s);
+#pragma unroll 2
+  for (int h = 0; h < heads; ++h) {
+    float x[16] = {};
+    if (pos >= 0) {
+      if constexpr (VEC) {
+        load8<T, true>(src + h * D + d0, x), load8<T, true>(src + h * D + d1, x + 8);
+        turn(a, d0, d1, c, s, x);
+      } else {
+        rotated16<T, false>(a, src + h * D, d0, d1, pos, x);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 16 / E; ++i) {
+      float f[E];
+#pragma unroll
+      for (int e = 0; e < E; ++e) f[e] = x[i * E + e];
+      *reinterpret_cast<U4*>(dst + h * D + (i < 8 / E ? d0 + i * E : d1 + i * E - 8)) = pack16<T>(f);
+    }
+  }
+}
+// rest: unit of the token's heads of K, then of V; `live`: there is such a unit.  Whole warps call it.
+template <typename T, int D, bool VEC>
+__device__ __forceinline__ void find_tops(const AppendArgs& a, unsigned* tops, int token, int rest, bool live) {
+  constexpr int kHeads = kHeadsOf<T>;
+  const int per_kind = units_of<T, D>(a.kv_heads);
+  const bool is_v = rest >= per_kind;
+  if (is_v) rest -= per_kind;
+  const int head0 = rest / (D / 16) * kHeads;
+  int d0, d1;
+  dims_of<VEC>(a, rest % (D / 16), d0, d1);
+  const int64_t pos = live ? a.positions[token] : -1;
+  const T* src = static_cast<const T*>(is_v ? a.v : a.k) + token * (is_v ? a.v_stride : a.k_stride) + head0 * D;
+  float c[8], s[8];
+  if (VEC && pos >= 0 && !is_v) angles_of(a, d0, d1, pos, c, s);
+#pragma unroll 2
+  for (int h = 0; h < kHeads; ++h) {
+    unsigned top = 0;
+    const bool some = pos >= 0 && head0 + h < a.kv_heads;
+    if (some) {
+      float x[16];
+      if (is_v || VEC) {
+        load8<T, VEC>(src + h * D + d0, x), load8<T, VEC>(src + h * D + d1, x + 8);
+        if (VEC && !is_v) turn(a, d0, d1, c, s, x);
+      } else {
+        rotated16<T, false>(a, src + h * D, d0, d1, pos, x);
+      }
+      top = largest(x);
+    }
+    top = row_max<D>(top);
+    if (some && rest % (D / 16) == 0) tops[(static_cast<int64_t>(token) * 2 + (is_v ? 1 : 0)) * a.kv_heads + head0 + h] = top;
+  }
+}
+
+// The scale behind the call from the one before and the bits of the largest |value|: NaN for anything that is not a finite number.
 __device__ __forceinline__ float grown(float before, unsigned top_bits, float per_top) {
   if (!isfinite(before) || top_bits >= 0x7f800000u) return __uint_as_float(0x7fffffffu);
   return fmaxf(before, __fmul_rn(__uint_as_float(top_bits), per_top));
 }
-template <typename C> __device__ __forceinline__ uint2 encode8(const float (&x)[8], float scale) {
-  float y[8];
-  const bool some = scale > 0.0f;  // not of a block of zeros, nor of one with a NaN
+// x / scale, correctly rounded, by Markstein's theorem: from the correctly rounded reciprocal r and a quotient q that is off by less than a unit
+// in the last place, q + r * (x - q * scale) is the rounded quotient, where nothing underflows.  x * r may be off by two, so it is corrected
+// twice.  x and a scale far from 1 are multiplied by a power of two first, which changes neither the quotient nor, for what can
+// become another code than 0, a bit of x.
+struct Divider {
+  float scale, r, lift;
+  bool some;  // not the scale of a block of zeros, nor NaN: all codes are 0
+};
+__device__ __forceinline__ Divider divider(float s) {
+  Divider d;
+  d.some = s > 0.0f;
+  d.lift = s > 1.2089258e24f ? 8.6736174e-19f : (s >= 8.2718061e-25f ? 1.0f : 1.2676506e30f);  // above 2^80: 2^-60, below 2^-80: 2^100
+  d.scale = d.some ? s * d.lift : 1.0f, d.r = __fdiv_rn(1.0f, d.scale);
+  return d;
+}
+__device__ __forceinline__ void divide16(const Divider& d, float (&x)[16]) {
+  if (d.lift != 1.0f) {  // also of a scale of 0 and of NaN
 #pragma unroll
-  for (int e = 0; e < 8; ++e) y[e] = some ? __fdiv_rn(x[e], scale) : 0.0f;
-  return make_uint2(Codec<C>::pack4(y), Codec<C>::pack4(y + 4));
+    for (int e = 0; e < 16; ++e) x[e] = d.some ? __fmul_rn(x[e], d.lift) : 0.0f;
+  }
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    float q = __fmul_rn(x[e], d.r);
+    q = __fmaf_rn(__fmaf_rn(-q, d.scale, x[e]), d.r, q);
+    x[e] = __fmaf_rn(__fmaf_rn(-q, d.scale, x[e]), d.r, q);
+  }
 }
 
-// Block (page, kvh) of K and V; s.token_of is filled and visible.  All threads call it.
+// A block of one call: where it is, and its scale before and behind the call.
+struct Block {
+  int64_t page;
+  int kvh;
+  bool is_v, move;  // move: rows that are not written anew are rounded to the grown scale
+  float ratio;
+  Divider by_scale;
+};
+__device__ __forceinline__ float* scale_of(const AppendArgs& a, const Block& b) { return (b.is_v ? a.v_scale : a.k_scale) + b.page * a.kv_heads + b.kvh; }
+__device__ __forceinline__ uint8_t* row_of(const AppendArgs& a, const Block& b, int row, int dim) {
+  return (b.is_v ? a.v_cache : a.k_cache) +
+         (a.hnd ? (b.page * a.kv_heads + b.kvh) * a.page_size + row : (b.page * a.page_size + row) * a.kv_heads + b.kvh) * dim;
+}
+template <typename C> __device__ __forceinline__ float rescale(Block& b, float was, bool begins, unsigned top) {
+  const float before = begins ? 0.0f : was, scale = grown(before, top, 1.0f / Codec<C>::kTop);
+  b.move = !begins && scale > before;
+  b.ratio = __fdiv_rn(before, scale);
+  b.by_scale = divider(scale);
+  return scale;
+}
+// Sixteen dims of row `row`: those of `token`, or of the codes that stand there.
+template <typename T, int D, bool VEC>
+__device__ __forceinline__ void row_values(const AppendArgs& a, bool is_v, int kvh, int token, int d0, int d1, float (&x)[16]) {
+  if (!is_v) rotated16<T, VEC>(a, static_cast<const T*>(a.k) + token * a.k_stride + kvh * D, d0, d1, a.positions[token], x);
+  else {
+    const T* head = static_cast<const T*>(a.v) + token * a.v_stride + kvh * D;
+    load8<T, VEC>(head + d0, x), load8<T, VEC>(head + d1, x + 8);
+  }
+}
 template <typename T, typename C, int D, bool VEC>
-__device__ __forceinline__ void write_block(const AppendArgs& a, BlockShared& s, int64_t page, int kvh) {
-  constexpr int kPerRow = D / 8, kRows = kThreads / kPerRow;  // threads of a row, rows at a time
-  constexpr int kKept = 2;                                    // passes whose values stay in registers
-  const int group = threadIdx.x / kPerRow, d0 = (threadIdx.x - group * kPerRow) * 8;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const T *k = static_cast<const T*>(a.k) + kvh * D, *v = static_cast<const T*>(a.v) + kvh * D;
-  const int64_t at_scale = page * a.kv_heads + kvh;
-  const float was_k = a.k_scale[at_scale], was_v = a.v_scale[at_scale];
-  auto values = [&](int token, float (&kx)[8], float (&vx)[8]) {
-    rotated8<T, VEC>(a, k + token * a.k_stride, d0, a.positions[token], kx);
-    load8<T, VEC>(v + token * a.v_stride + d0, vx);
-  };
-  float kk[kKept][8], vv[kKept][8];
-  unsigned top_k = 0, top_v = 0;
+__device__ __forceinline__ void write_row(const AppendArgs& a, const Block& b, int row, int token, int d0, int d1) {
+  if (token < 0 && !b.move) return;
+  uint8_t* to = row_of(a, b, row, D);
+  uint2 *at0 = reinterpret_cast<uint2*>(to + d0), *at1 = reinterpret_cast<uint2*>(to + d1);
+  float x[16];
+  if (token >= 0) {
+    row_values<T, D, VEC>(a, b.is_v, b.kvh, token, d0, d1, x);
+    divide16(b.by_scale, x);
+  } else {
+    const uint2 c0 = *at0, c1 = *at1;
+    Codec<C>::unpack4(c0.x, x), Codec<C>::unpack4(c0.y, x + 4), Codec<C>::unpack4(c1.x, x + 8), Codec<C>::unpack4(c1.y, x + 12);
 #pragma unroll
-  for (int i = 0; i < kKept; ++i) {
-    const int row = group + i * kRows;
-    if (row < a.page_size && s.token_of[row] >= 0) {
-      values(s.token_of[row], kk[i], vv[i]);
-      top_k = largest8(top_k, kk[i]), top_v = largest8(top_v, vv[i]);
-    }
+    for (int e = 0; e < 16; ++e) x[e] = __fmul_rn(x[e], b.ratio);
   }
-  for (int row = group + kKept * kRows; row < a.page_size; row += kRows) {
-    if (s.token_of[row] < 0) continue;
-    float kx[8], vx[8];
-    values(s.token_of[row], kx, vx);
-    top_k = largest8(top_k, kx), top_v = largest8(top_v, vx);
+  *at0 = make_uint2(Codec<C>::pack4(x), Codec<C>::pack4(x + 4));
+  *at1 = make_uint2(Codec<C>::pack4(x + 8), Codec<C>::pack4(x + 12));
+}
+// The mean of four dims of a block of K, whose codes are all written.
+template <typename C, int D> __device__ __forceinline__ void write_mean(const AppendArgs& a, const Block& b, int d) {
+  int sums[4] = {};
+#pragma unroll 8
+  for (int row = 0; row < a.page_size; ++row) {
+    float f[4];
+    Codec<C>::unpack4(__ldcg(reinterpret_cast<const uint32_t*>(row_of(a, b, row, D) + d)), f);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sums[e] += static_cast<int>(f[e] * Codec<C>::kUnits);
   }
-  top_k = __reduce_max_sync(0xffffffffu, top_k), top_v = __reduce_max_sync(0xffffffffu, top_v);
-  if (lane == 0) s.top_k[warp] = top_k, s.top_v[warp] = top_v;
-  const bool means = a.k_mean != nullptr && s.token_of[a.page_size - 1] >= 0;
-  const bool begins = s.token_of[0] >= 0;
-  for (int i = threadIdx.x; i < D; i += kThreads) s.sums[i] = 0;
-  __syncthreads();
+  uint32_t packed = 0;
 #pragma unroll
-  for (int w = 0; w < kThreads / 32; ++w) top_k = max(top_k, s.top_k[w]), top_v = max(top_v, s.top_v[w]);
-  const float before_k = begins ? 0.0f : was_k, before_v = begins ? 0.0f : was_v;
-  const float scale_k = grown(before_k, top_k, 1.0f / Codec<C>::kTop), scale_v = grown(before_v, top_v, 1.0f / Codec<C>::kTop);
-  if (threadIdx.x == 0) a.k_scale[at_scale] = scale_k, a.v_scale[at_scale] = scale_v;
-  const bool move_k = !begins && scale_k > before_k, move_v = !begins && scale_v > before_v;
-  const float ratio_k = __fdiv_rn(before_k, scale_k), ratio_v = __fdiv_rn(before_v, scale_v);
-
-  int sums[8] = {};
-  auto moved = [](uint2 old, float ratio) {
-    float f[8];
-    Codec<C>::unpack4(old.x, f), Codec<C>::unpack4(old.y, f + 4);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = __fmul_rn(f[e], ratio);
-    return make_uint2(Codec<C>::pack4(f), Codec<C>::pack4(f + 4));
-  };
-  auto finish_row = [&](int row, const float (&kx)[8], const float (&vx)[8]) {
-    const bool fresh = s.token_of[row] >= 0;
-    const int64_t at = (a.hnd ? (page * a.kv_heads + kvh) * a.page_size + row : (page * a.page_size + row) * a.kv_heads + kvh) * D + d0;
-    uint2 *kc = reinterpret_cast<uint2*>(a.k_cache + at), *vc = reinterpret_cast<uint2*>(a.v_cache + at);
-    uint2 code = {};
-    if (fresh) {
-      *kc = code = encode8<C>(kx, scale_k);
-      *vc = encode8<C>(vx, scale_v);
-    } else {
-      if (move_k || means) code = *kc;
-      if (move_k) *kc = code = moved(code, ratio_k);
-      if (move_v) *vc = moved(*vc, ratio_v);
-    }
-    if (means) {
-      float f[8];
-      Codec<C>::unpack4(code.x, f), Codec<C>::unpack4(code.y, f + 4);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) sums[e] += static_cast<int>(f[e] * Codec<C>::kUnits);
-    }
-  };
-#pragma unroll
-  for (int i = 0; i < kKept; ++i)
-    if (group + i * kRows < a.page_size) finish_row(group + i * kRows, kk[i], vv[i]);
-  for (int row = group + kKept * kRows; row < a.page_size; row += kRows) {
-    float kx[8], vx[8];
-    if (s.token_of[row] >= 0) values(s.token_of[row], kx, vx);
-    finish_row(row, kx, vx);
+  for (int e = 0; e < 4; ++e) {
+    const float m = rintf(__fmul_rn(static_cast<float>(sums[e]), a.mean_unit));
+    packed |= (static_cast<uint32_t>(static_cast<int>(fminf(fmaxf(m, -127.0f), 127.0f))) & 0xffu) << (8 * e);
   }
-  if (!means) return;  // the same for all threads
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-#pragma unroll
-    for (int sh = kPerRow; sh < 32; sh <<= 1) sums[e] += __shfl_xor_sync(0xffffffffu, sums[e], sh);
-    if (lane < kPerRow || kPerRow == 32) atomicAdd(&s.sums[d0 + e], sums[e]);
-  }
-  __syncthreads();
-  for (int d = threadIdx.x; d < D; d += kThreads) {
-    const float m = rintf(__fmul_rn(static_cast<float>(s.sums[d]), a.mean_unit));
-    a.k_mean[at_scale * D + d] = static_cast<int8_t>(static_cast<int>(fminf(fmaxf(m, -127.0f), 127.0f)));
-  }
+  *reinterpret_cast<uint32_t*>(a.k_mean + (b.page * a.kv_heads + b.kvh) * D + d) = packed;
 }
 
-// Batches of up to kSmallBatch tokens: y < kv_heads: the block of the token's page, if no token before it has the same page; the
-// other y rotate Q.
+// Batches of up to kSmallBatch tokens: a CTA has four of the 2 * kv_heads blocks of K and V of the token's page, if no token before it has
+// the same page; the CTAs behind those (`block_rows` of them) rotate Q.
 template <typename T, typename C, int D, bool VEC>
 __global__ void __launch_bounds__(kThreads)
-kv8_append_kernel(const __grid_constant__ AppendArgs a) {
-  __shared__ BlockShared s;
+kv8_append_kernel(const __grid_constant__ AppendArgs a, int block_rows) {
+  extern __shared__ int token_of[];  // [page_size]
   __shared__ int64_t pages[kSmallBatch];
   pdl_launch_dependents();
   pdl_wait();  // q, k, v may be the preceding kernel's output; the caches may still be read by it
-  const int token = blockIdx.x, kvh = blockIdx.y;
-  if (kvh >= a.kv_heads) {
-    rotate_q<T, D, VEC>(a, token, (kvh - a.kv_heads) * kThreads + threadIdx.x);
+  const int token = blockIdx.x, part = blockIdx.y;
+  if (part >= block_rows) {
+    const int unit = (part - block_rows) * kThreads + threadIdx.x;
+    if (unit < units_of<T, D>(a.q_heads)) rotate_q<T, D, VEC>(a, token, unit);
     return;
   }
   const int other = threadIdx.x;
@@ -302,84 +369,163 @@ kv8_append_kernel(const __grid_constant__ AppendArgs a) {
     }
     pages[other] = page;
   }
-  for (int i = threadIdx.x; i < a.page_size; i += kThreads) s.token_of[i] = -1;
+  for (int i = threadIdx.x; i < a.page_size; i += kThreads) token_of[i] = -1;
   __syncthreads();
   const int64_t mine = pages[token];
   if (__syncthreads_or(mine < 0 || (other < token && page == mine))) return;
-  if (other < a.tokens && page == mine) atomicMax(&s.token_of[row], other);
+  if (other < a.tokens && page == mine) atomicMax(&token_of[row], other);
   __syncthreads();
-  write_block<T, C, D, VEC>(a, s, mine, kvh);
+  const int head = part * (kThreads / 32) + (threadIdx.x >> 5);  // of K, then of V
+  if (head >= 2 * a.kv_heads) return;
+  Block b;
+  b.page = mine, b.is_v = head >= a.kv_heads, b.kvh = b.is_v ? head - a.kv_heads : head;
+  constexpr int kPerRow = D / 16, kRows = 32 / kPerRow;  // lanes of a row, rows at a time
+  const int lane = threadIdx.x & 31, group = lane / kPerRow;
+  int d0, d1;
+  dims_of<VEC>(a, lane - group * kPerRow, d0, d1);
+  float* scale_at = scale_of(a, b);
+  const float was = *scale_at;
+  unsigned top = 0;
+#pragma unroll 1
+  for (int r = group; r < a.page_size; r += kRows)
+    if (token_of[r] >= 0) {
+      float x[16];
+      row_values<T, D, VEC>(a, b.is_v, b.kvh, token_of[r], d0, d1, x);
+      top = max(top, largest(x));
+    }
+  top = __reduce_max_sync(0xffffffffu, top);
+  const float scale = rescale<C>(b, was, token_of[0] >= 0, top);
+  if (lane == 0) *scale_at = scale;  // every lane has read it: the reduction stands between
+#pragma unroll 1
+  for (int r = group; r < a.page_size; r += kRows) write_row<T, C, D, VEC>(a, b, r, token_of[r], d0, d1);  // values again, from L1
+  if (b.is_v || a.k_mean == nullptr || token_of[a.page_size - 1] < 0) return;  // the same for all lanes
+  __syncwarp();
+  for (int d = lane * 4; d < D; d += 32 * 4) write_mean<C, D>(a, b, d);
 }
 
-// Longer batches, first launch: rotates Q, and enters every token's page into the table.
+// Longer batches, first launch: the first `entries` CTAs enter every token's page into the table, the next `q_blocks` rotate Q, the others
+// find the largest values of K and V.
 template <typename T, int D, bool VEC>
 __global__ void __launch_bounds__(kThreads)
-kv8_group_kernel(const __grid_constant__ AppendArgs a, const __grid_constant__ Groups g) {
+kv8_group_kernel(const __grid_constant__ AppendArgs a, const __grid_constant__ Groups g, unsigned entries, unsigned q_blocks) {
   pdl_launch_dependents();
   pdl_wait();
-  const int token = blockIdx.x;
-  if (blockIdx.y == 0 && threadIdx.x == 0) {
-    const int64_t pos = a.positions[token];
-    const int64_t physical = pos >= 0 ? a.page_table[a.sequence_ids[token] * a.max_pages + pos / a.page_size] : -1;
-    int slot = -1;
-    if (physical >= 0) {
-      const unsigned long long page = static_cast<unsigned long long>(physical);
-      unsigned at = static_cast<unsigned>((page * 0x9e3779b97f4a7c15ull) >> 32) & g.mask;
-      for (unsigned tries = 0; tries <= g.mask; ++tries, at = (at + 1) & g.mask) {  // half of the entries stay free
-        const unsigned long long found = atomicCAS(&g.page[at], ~0ull, page);
-        if (found == ~0ull) g.list[atomicAdd(g.count, 1) + 1] = static_cast<int>(at);
-        if (found == ~0ull || found == page) {
-          slot = static_cast<int>(at);
-          break;
-        }
-      }
-      if (slot >= 0) {
-        atomicMin(&g.first[slot], static_cast<unsigned>(token));
-        atomicMax(&g.last[slot], token);
+  if (blockIdx.x >= entries) {
+    const bool is_q = blockIdx.x < entries + q_blocks;
+    const int64_t first = static_cast<int64_t>(blockIdx.x - (is_q ? entries : entries + q_blocks)) * kThreads;  // unit of thread 0
+    const int per_token = is_q ? units_of<T, D>(a.q_heads) : 2 * units_of<T, D>(a.kv_heads);
+    int token = static_cast<int>(first / per_token);
+    int unit = static_cast<int>(first - static_cast<int64_t>(token) * per_token) + threadIdx.x;
+    const int further = unit / per_token;
+    token += further, unit -= further * per_token;
+    if (!is_q) find_tops<T, D, VEC>(a, g.tops, token < a.tokens ? token : 0, unit, token < a.tokens);
+    else if (token < a.tokens) rotate_q<T, D, VEC>(a, token, unit);
+    return;
+  }
+  const int token = blockIdx.x * kThreads + threadIdx.x;
+  if (token >= a.tokens) return;
+  const int64_t pos = a.positions[token];
+  const int64_t logical = pos / a.page_size;
+  const int64_t physical = pos >= 0 ? a.page_table[a.sequence_ids[token] * a.max_pages + logical] : -1;
+  g.row_of[token] = static_cast<uint16_t>(pos - logical * a.page_size);
+  int slot = -1;
+  if (physical >= 0) {
+    const unsigned long long page = static_cast<unsigned long long>(physical);
+    unsigned at = static_cast<unsigned>((page * 0x9e3779b97f4a7c15ull) >> 32) & g.mask;
+    for (unsigned tries = 0; tries <= g.mask; ++tries, at = (at + 1) & g.mask) {  // half of the entries stay free
+      const unsigned long long found = atomicCAS(&g.page[at], ~0ull, page);
+      if (found == ~0ull) g.list[atomicAdd(g.count, 1) + 1] = static_cast<int>(at);
+      if (found == ~0ull || found == page) {
+        slot = static_cast<int>(at);
+        break;
       }
     }
-    g.slot_of[token] = slot;
+    if (slot >= 0) {
+      atomicMin(&g.first[slot], static_cast<unsigned>(token));
+      atomicMax(&g.last[slot], token);
+    }
   }
-  rotate_q<T, D, VEC>(a, token, blockIdx.y * kThreads + threadIdx.x);
+  g.slot_of[token] = slot;
 }
 
-// Second launch: the blocks of the pages in the table, in turn.
+// Second launch: CTAs take four blocks of a page in the table in turn.  A warp finds the scale of one, then all threads write the rows of
+// all four.
 template <typename T, typename C, int D, bool VEC>
 __global__ void __launch_bounds__(kThreads)
-kv8_blocks_kernel(const __grid_constant__ AppendArgs a, const __grid_constant__ Groups g) {
-  __shared__ BlockShared s;
+kv8_blocks_kernel(const __grid_constant__ AppendArgs a, const __grid_constant__ Groups g, unsigned parts) {
+  constexpr int kWarps = kThreads / 32, kPerRow = D / 16;
+  extern __shared__ int token_of[];  // [page_size]
+  __shared__ Block blocks[kWarps];
   pdl_launch_dependents();
   pdl_wait();
-  const int64_t items = static_cast<int64_t>(*g.count + 1) * a.kv_heads;
-  for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-    const int entry = static_cast<int>(item / a.kv_heads), kvh = static_cast<int>(item - static_cast<int64_t>(entry) * a.kv_heads);
+  const unsigned part = blockIdx.x % parts;  // of a page's blocks; the grid: a multiple of them
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, heads = 2 * a.kv_heads;
+  const int head = part * kWarps + warp, some = heads - static_cast<int>(part) * kWarps < kWarps ? heads - part * kWarps : kWarps;
+  int d0, d1;
+  dims_of<VEC>(a, threadIdx.x % kPerRow, d0, d1);
+  for (unsigned entry = blockIdx.x / parts; entry <= g.mask; entry += gridDim.x / parts) {
     const int slot = g.list[entry];
-    for (int i = threadIdx.x; i < a.page_size; i += kThreads) s.token_of[i] = -1;
+    if (slot < 0) return;  // behind the last one; the same for all threads
+    for (int i = threadIdx.x; i < a.page_size; i += kThreads) token_of[i] = -1;
+    const int first = static_cast<int>(g.first[slot]), last = g.last[slot];
+    Block b;
+    b.page = static_cast<int64_t>(g.page[slot]), b.is_v = head >= a.kv_heads, b.kvh = b.is_v ? head - a.kv_heads : head;
+    const float was = head < heads ? *scale_of(a, b) : 0.0f;
     __syncthreads();
-    const int last = g.last[slot];
-    for (int t = static_cast<int>(g.first[slot]) + threadIdx.x; t <= last; t += kThreads)
-      if (g.slot_of[t] == slot) atomicMax(&s.token_of[static_cast<int>(a.positions[t] % a.page_size)], t);
+    for (int t = first + threadIdx.x; t <= last; t += kThreads) {
+      const int row = g.row_of[t];
+      if (g.slot_of[t] == slot) atomicMax(&token_of[row], t);
+    }
     __syncthreads();
-    write_block<T, C, D, VEC>(a, s, static_cast<int64_t>(g.page[slot]), kvh);
-    __syncthreads();  // its shared memory is free again
+    if (head < heads) {
+      unsigned top = 0;
+      for (int r = lane; r < a.page_size; r += 32)
+        if (token_of[r] >= 0) top = max(top, g.tops[static_cast<int64_t>(token_of[r]) * heads + head]);
+      top = __reduce_max_sync(0xffffffffu, top);
+      const float scale = rescale<C>(b, was, token_of[0] >= 0, top);
+      if (lane == 0) {
+        *scale_of(a, b) = scale;
+        blocks[warp] = b;
+      }
+    }
+    __syncthreads();
+    // rows of one block after the other: neighbours in HND; in NHD the blocks' rows stand side by side
+    for (int i = threadIdx.x / kPerRow; i < a.page_size * some; i += kThreads / kPerRow) {
+      const int of = i / a.page_size, row = i - of * a.page_size;
+      write_row<T, C, D, VEC>(a, blocks[of], row, token_of[row], d0, d1);
+    }
+    const bool means = a.k_mean != nullptr && token_of[a.page_size - 1] >= 0 && static_cast<int>(part) * kWarps < a.kv_heads;
+    __syncthreads();  // the codes are written
+    if (means)
+      for (int i = threadIdx.x; i < some * (D / 4); i += kThreads)
+        if (!blocks[i / (D / 4)].is_v) write_mean<C, D>(a, blocks[i / (D / 4)], i % (D / 4) * 4);
+    __syncthreads();  // shared memory is free again
   }
 }
 
 template <typename T, typename C, int D, bool VEC>
 int launch_append(const AppendArgs& a, void* scratch, cudaStream_t stream) {
-  const int64_t q_blocks = (static_cast<int64_t>(a.q_heads) * (D / 8) + kThreads - 1) / kThreads;
-  if (q_blocks + a.kv_heads > 65535) return XDK_ERR_LIMIT;
-  if (a.tokens <= kSmallBatch)
-    return launch_dependent(kv8_append_kernel<T, C, D, VEC>, dim3(static_cast<unsigned>(a.tokens), static_cast<unsigned>(a.kv_heads + q_blocks)),
-                            dim3(kThreads), 0, stream, a);
-  const Groups g = groups_at(scratch, a.tokens);
-  if (int st = note_launch(cudaMemsetAsync(scratch, 0xff, group_bytes(a.tokens), stream))) return st;
-  if (int st = launch_opts(kv8_group_kernel<T, D, VEC>, dim3(static_cast<unsigned>(a.tokens), static_cast<unsigned>(q_blocks)), dim3(kThreads), 0,
-                           stream, 1u, false, a, g))
+  const int64_t q_units = units_of<T, D>(a.q_heads), heads = 2 * static_cast<int64_t>(a.kv_heads), warps = kThreads / 32;
+  const int64_t parts = (heads + warps - 1) / warps;
+  const size_t map = static_cast<size_t>(a.page_size) * 4;
+  if (a.tokens <= kSmallBatch) {
+    const int64_t rows = parts + (q_units + kThreads - 1) / kThreads;
+    if (rows > 65535) return XDK_ERR_LIMIT;
+    return launch_dependent(kv8_append_kernel<T, C, D, VEC>, dim3(static_cast<unsigned>(a.tokens), static_cast<unsigned>(rows)), dim3(kThreads), map,
+                            stream, a, static_cast<int>(parts));
+  }
+  const Groups g = groups_at(scratch, a.tokens, a.kv_heads);
+  if (int st = note_launch(cudaMemsetAsync(scratch, 0xff, cleared_bytes(a.tokens), stream))) return st;
+  const int64_t entries = (a.tokens + kThreads - 1) / kThreads, q_blocks = (a.tokens * q_units + kThreads - 1) / kThreads;
+  const int64_t kv_blocks = (a.tokens * 2 * units_of<T, D>(a.kv_heads) + kThreads - 1) / kThreads;
+  if (entries + q_blocks + kv_blocks > 2147483647LL) return XDK_ERR_LIMIT;
+  if (int st = launch_opts(kv8_group_kernel<T, D, VEC>, dim3(static_cast<unsigned>(entries + q_blocks + kv_blocks)), dim3(kThreads), 0, stream, 1u,
+                           false, a, g, static_cast<unsigned>(entries), static_cast<unsigned>(q_blocks)))
     return st;
-  const int64_t most = static_cast<int64_t>(a.tokens) * a.kv_heads, wave = static_cast<int64_t>(sm_count()) * 8;
-  return launch_opts(kv8_blocks_kernel<T, C, D, VEC>, dim3(static_cast<unsigned>(most < wave ? most : wave)), dim3(kThreads), 0, stream, 1u, true,
-                     a, g);
+  // as many CTAs as there can be work for, or the SMs hold
+  const int64_t wave = (static_cast<int64_t>(sm_count()) * 8 + parts - 1) / parts;
+  return launch_opts(kv8_blocks_kernel<T, C, D, VEC>, dim3(static_cast<unsigned>((a.tokens < wave ? a.tokens : wave) * parts)), dim3(kThreads), map,
+                     stream, 1u, true, a, g, static_cast<unsigned>(parts));
 }
 
 template <typename T, typename C>
@@ -401,8 +547,9 @@ int dispatch_append(int64_t d, const AppendArgs& a, void* scratch, cudaStream_t 
 }  // namespace
 }  // namespace xdk
 
-extern "C" size_t xdk_kv8_append_scratch_bytes(int64_t tokens) {
-  return tokens <= xdk::kSmallBatch || tokens > (1LL << 26) ? 0 : xdk::group_bytes(tokens);
+extern "C" size_t xdk_kv8_append_scratch_bytes(int64_t tokens, int64_t kv_heads) {
+  if (tokens <= xdk::kSmallBatch || tokens > (1LL << 26) || kv_heads < 1 || kv_heads > 65535) return 0;
+  return xdk::group_bytes(tokens, kv_heads);
 }
 
 extern "C" int xdk_kv8_append(const void* q, const void* k, const void* v, const float* cos, const float* sin, const int64_t* positions,
@@ -422,7 +569,7 @@ extern "C" int xdk_kv8_append(const void* q, const void* k, const void* v, const
   if (!aligned16(q_out) || !aligned16(k_cache) || !aligned16(v_cache)) return XDK_ERR_ARG;
   if (!kv8_head_dim(head_dim) || q_heads > 65535 || cos_width > 2147483647LL) return XDK_ERR_LIMIT;
   if (int st = kv8_limits(tokens, kv_heads, max_pages_per_seq, page_size)) return st;
-  const size_t need = xdk_kv8_append_scratch_bytes(tokens);
+  const size_t need = xdk_kv8_append_scratch_bytes(tokens, kv_heads);
   if (need > 0 && (!scratch || scratch_bytes < need || !aligned16(scratch))) return XDK_ERR_ARG;
   if (codes != XDK_KV8_INT8 && codes != XDK_KV8_E4M3) return XDK_ERR_ARG;
   if (dtype != XDK_F32 && dtype != XDK_BF16 && dtype != XDK_F16) return XDK_ERR_ARG;

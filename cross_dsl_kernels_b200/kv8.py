@@ -170,7 +170,7 @@ def rope_gqa_paged_kv8_append(q, k, v, cos, sin, positions, page_table, sequence
         lib = _native.lib()
         q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         # the groups of a long batch by page: a fresh block per call, as the scratch of the other ops
-        need = lib.xdk_kv8_append_scratch_bytes(tokens)
+        need = lib.xdk_kv8_append_scratch_bytes(tokens, kv_heads)
         scratch = torch.empty(need, device=q.device, dtype=torch.uint8) if need else None
         status = lib.xdk_kv8_append(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), cos.data_ptr(), sin.data_ptr(), positions.data_ptr(), page_table.data_ptr(),

@@ -317,7 +317,7 @@ XDK_API int xdk_swiglu_peer(const void* upgate, const xdk_peer_out* out_dst, int
  *     If the last row is in W, the mean of the block's codes as int8, in units of scale, or of scale * 448 / 127 for e4m3.
  *   So a page begins anew when its first position is written.  A scale is NaN, and the block reads as NaN, from when it is given a value
  *   that is not finite until then.  positions[t] < 0 (padding): nothing is written, q_out of the token is 0.  q, k, v are strided as there,
- *   q_out is contiguous; k_mean may be NULL (no means).  scratch: xdk_kv8_append_scratch_bytes(tokens) bytes (0 for
+ *   q_out is contiguous; k_mean may be NULL (no means).  scratch: xdk_kv8_append_scratch_bytes bytes (0 for
  *   small batches), content undefined, not shared by calls that may overlap on the GPU; one memset and two launches then, one launch else.
  * xdk_kv8_decode_attention: xdk_paged_decode_attention_ws for this cache: any q_heads / kv_heads up to 8; softmax and sums in FP32; a context
  *   of no positions (positions[t] < 0) gives 0.  Two launches.  scratch: xdk_kv8_decode_attention_scratch_bytes(..., the same context_hint)
@@ -332,7 +332,7 @@ XDK_API int xdk_swiglu_peer(const void* upgate, const xdk_peer_out* out_dst, int
  *   xdk_kv8_sparse_attention_scratch_bytes.
  */
 typedef enum xdk_kv8_codes { XDK_KV8_INT8 = 0, XDK_KV8_E4M3 = 1 } xdk_kv8_codes;
-XDK_API size_t xdk_kv8_append_scratch_bytes(int64_t tokens);
+XDK_API size_t xdk_kv8_append_scratch_bytes(int64_t tokens, int64_t kv_heads);
 XDK_API int xdk_kv8_append(const void* q, const void* k, const void* v, const float* cos, const float* sin, const int64_t* positions,
                    const int64_t* page_table, const int64_t* sequence_ids, void* q_out, void* k_cache, void* v_cache,
                    float* k_scale, float* v_scale, int8_t* k_mean, int64_t tokens, int64_t q_heads, int64_t kv_heads,
