@@ -7,9 +7,10 @@
 // the same whatever computes it.  One choice per token and KV head: the query heads that share it read its pages together.
 //
 // One CTA per (token, KV head).  Scores: mma.m16n8k32 on bytes, 16 pages as rows, the heads of the group as columns; a thread
-// loads a quarter of two pages' means with 16-byte loads, and the codes of q stand in registers in the same order of dims.  The scores
-// stay in shared memory as sortable integers; four passes over their bytes find the value of the last one chosen, a fifth writes
-// the pages in order.  Bound: short contexts by the chain of launches and barriers, long ones by the reads of the means.
+// loads a quarter of two pages' means with 16-byte loads, those of a few blocks of pages at a time, and the codes of q stand in
+// registers in the same order of dims.  The scores stay in shared memory as sortable integers; up to three passes over 11, 11 and 10 bits of
+// them find the value of the last one chosen (two, mostly: no other has its first 22 bits), one more writes the pages in order.
+// Bound: short contexts by the chain of loads and barriers, long ones by the latency of the reads of the means.
 #include <math.h>
 
 #include "kv8.cuh"
@@ -18,6 +19,7 @@ namespace xdk {
 namespace {
 
 constexpr int kSelThreads = 512, kSelWarps = kSelThreads / 32;
+constexpr int kBins = 2048, kBinsEach = kBins / kSelThreads;
 constexpr int64_t kMaxCandidates = 51200;  // keys in shared memory
 
 struct SelectArgs {
@@ -49,8 +51,8 @@ kv8_select_kernel(const __grid_constant__ SelectArgs a) {
   extern __shared__ uint32_t keys[];
   __shared__ __align__(16) uint32_t codes[8][D / 4];
   __shared__ float unit[8];
-  __shared__ unsigned bins[256];
-  __shared__ unsigned warp_sum[8], chosen[2];
+  __shared__ unsigned bins[kBins];
+  __shared__ unsigned warp_sum[kSelWarps], chosen[3];
   __shared__ int warp_above[kSelWarps], warp_equal[kSelWarps];
 
   pdl_launch_dependents();
@@ -69,6 +71,10 @@ kv8_select_kernel(const __grid_constant__ SelectArgs a) {
   const int want = a.top_pages - 1;  // of the pages in front of the last one
   if (last <= want) {
     for (int i = tid; i < a.top_pages; i += kSelThreads) out[i] = i <= last ? i : -1;
+    return;
+  }
+  if (want == 0) {
+    if (tid == 0) out[0] = last;
     return;
   }
   const int64_t* table = a.page_table + a.sequence_ids[token] * a.max_pages;
@@ -102,87 +108,113 @@ kv8_select_kernel(const __grid_constant__ SelectArgs a) {
   for (int w = 0; w < kWords; ++w) b[w] = codes[row][quad * kWords + w];
   const float unit0 = unit[2 * quad], unit1 = unit[2 * quad + 1];
   const bool live0 = 2 * quad < group, live1 = 2 * quad + 1 < group;
-  for (int base = warp * 16; base < last; base += kSelWarps * 16) {
-    const int p0 = base + row, p1 = p0 + 8;
-    const int64_t block0 = (p0 < last ? table[p0] : table[base]) * a.kv_heads + kvh, block1 = (p1 < last ? table[p1] : table[base]) * a.kv_heads + kvh;
-    uint32_t m0[kWords], m1[kWords];
+  constexpr int kAtOnce = D <= 128 ? 4 : 2;  // blocks of 16 pages whose loads are on their way together
+  for (int base0 = warp * 16; base0 < last; base0 += kSelWarps * 16 * kAtOnce) {
+    int64_t block[kAtOnce][2];
+    uint32_t m[kAtOnce][2][kWords];
+    float scale[kAtOnce][2];
 #pragma unroll
-    for (int w = 0; w < kWords; w += 4) {
-      const U4 v0 = ld_ordered_stream16(a.k_mean + block0 * D + quad * (D / 4) + w * 4);
-      const U4 v1 = ld_ordered_stream16(a.k_mean + block1 * D + quad * (D / 4) + w * 4);
-      m0[w] = v0.x, m0[w + 1] = v0.y, m0[w + 2] = v0.z, m0[w + 3] = v0.w;
-      m1[w] = v1.x, m1[w + 1] = v1.y, m1[w + 2] = v1.z, m1[w + 3] = v1.w;
+    for (int u = 0; u < kAtOnce; ++u)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const int p = base0 + u * kSelWarps * 16 + row + r * 8;
+        block[u][r] = table[p < last ? p : last - 1] * a.kv_heads + kvh;  // dead rows: one that is read anyway
+      }
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        if (base0 + u * kSelWarps * 16 >= last) continue;
+#pragma unroll
+        for (int w = 0; w < kWords; w += 4) {
+          const U4 v = ld_ordered_stream16(a.k_mean + block[u][r] * D + quad * (D / 4) + w * 4);
+          m[u][r][w] = v.x, m[u][r][w + 1] = v.y, m[u][r][w + 2] = v.z, m[u][r][w + 3] = v.w;
+        }
+        scale[u][r] = a.k_scale[block[u][r]];
+      }
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u) {
+      const int p0 = base0 + u * kSelWarps * 16 + row, p1 = p0 + 8;
+      if (p0 - row >= last) break;  // the same for the warp
+      int dot[4] = {};
+#pragma unroll
+      for (int w = 0; w < kWords; w += 2) mma_s8(dot, m[u][0][w], m[u][1][w], m[u][0][w + 1], m[u][1][w + 1], b[w], b[w + 1]);
+      float s[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float x = live0 ? __fmul_rn(static_cast<float>(dot[2 * e]), unit0) : -INFINITY;
+        const float y = live1 ? __fmul_rn(static_cast<float>(dot[2 * e + 1]), unit1) : -INFINITY;
+        s[e] = fmaxf(x, y);
+#pragma unroll
+        for (int sh = 1; sh < 4; sh <<= 1) s[e] = fmaxf(s[e], __shfl_xor_sync(0xffffffffu, s[e], sh));
+      }
+      if (quad == 0 && p0 < last) keys[p0] = key_of(__fmul_rn(s[0], scale[u][0]));
+      if (quad == 1 && p1 < last) keys[p1] = key_of(__fmul_rn(s[1], scale[u][1]));
     }
-    const float scale0 = a.k_scale[block0], scale1 = a.k_scale[block1];
-    int dot[4] = {};
-#pragma unroll
-    for (int w = 0; w < kWords; w += 2) mma_s8(dot, m0[w], m1[w], m0[w + 1], m1[w + 1], b[w], b[w + 1]);
-    float s[2];
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const float x = live0 ? __fmul_rn(static_cast<float>(dot[2 * e]), unit0) : -INFINITY;
-      const float y = live1 ? __fmul_rn(static_cast<float>(dot[2 * e + 1]), unit1) : -INFINITY;
-      s[e] = fmaxf(x, y);
-#pragma unroll
-      for (int sh = 1; sh < 4; sh <<= 1) s[e] = fmaxf(s[e], __shfl_xor_sync(0xffffffffu, s[e], sh));
-    }
-    if (quad == 0 && p0 < last) keys[p0] = key_of(__fmul_rn(s[0], scale0));
-    if (quad == 1 && p1 < last) keys[p1] = key_of(__fmul_rn(s[1], scale1));
   }
 
-  // ---- the key of the last one chosen, byte by byte from the top; `left`: how many of the keys that agree so far are wanted
+  // ---- the key of the last one chosen, from its high bits down; `left`: how many of the keys that agree so far are wanted
   uint32_t prefix = 0;
   unsigned left = static_cast<unsigned>(want);
-  if (want > 0) {
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      if (tid < 256) bins[tid] = 0;
-      __syncthreads();
-      const uint32_t mask = shift == 24 ? 0u : 0xffffffffu << (shift + 8);
-      for (int i = tid; i < last; i += kSelThreads)
-        if ((keys[i] & mask) == prefix) atomicAdd(&bins[keys[i] >> shift & 255u], 1u);
-      __syncthreads();
-      unsigned mine = 0, upto = 0;
-      if (tid < 256) {  // thread t: bin 255 - t; keys in it and in those above
-        mine = upto = bins[255 - tid];
+  bool exact = false;  // all bits of prefix are known; else all keys that agree with the known ones are wanted
+#pragma unroll 1
+  for (int pass = 0; pass < 3; ++pass) {
+    const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0), bits = pass == 2 ? 10 : 11;
 #pragma unroll
-        for (int sh = 1; sh < 32; sh <<= 1) {
-          const unsigned v = __shfl_up_sync(0xffffffffu, upto, sh);
-          if (lane >= sh) upto += v;
-        }
-        if (lane == 31) warp_sum[warp] = upto;
-      }
-      __syncthreads();
-      if (tid < 256) {
-        for (int w = 0; w < warp; ++w) upto += warp_sum[w];
-        if (upto - mine < left && left <= upto) chosen[0] = 255u - tid, chosen[1] = left - (upto - mine);
-      }
-      __syncthreads();
-      prefix |= chosen[0] << shift, left = chosen[1];
-    }
-  } else {
-    prefix = 0xffffffffu, left = 0;
+    for (int i = 0; i < kBinsEach; ++i) bins[i * kSelThreads + tid] = 0;
     __syncthreads();
+    const uint32_t mask = pass == 0 ? 0u : 0xffffffffu << (shift + bits);
+    for (int i = tid; i < last; i += kSelThreads)
+      if ((keys[i] & mask) == prefix) atomicAdd(&bins[keys[i] >> shift & ((1u << bits) - 1u)], 1u);
+    __syncthreads();
+    // thread t: kBinsEach bins from the top down; keys in them and in those above
+    unsigned mine[kBinsEach], upto = 0;
+#pragma unroll
+    for (int i = 0; i < kBinsEach; ++i) upto += mine[i] = bins[kBins - 1 - (tid * kBinsEach + i)];
+    const unsigned own = upto;
+#pragma unroll
+    for (int sh = 1; sh < 32; sh <<= 1) {
+      const unsigned v = __shfl_up_sync(0xffffffffu, upto, sh);
+      if (lane >= sh) upto += v;
+    }
+    if (lane == 31) warp_sum[warp] = upto;
+    __syncthreads();
+    for (int w = 0; w < warp; ++w) upto += warp_sum[w];
+    unsigned above = upto - own;
+    if (above < left && left <= upto) {
+#pragma unroll
+      for (int i = 0; i < kBinsEach; ++i) {
+        if (above < left && left <= above + mine[i]) chosen[0] = kBins - 1 - (tid * kBinsEach + i), chosen[1] = left - above, chosen[2] = mine[i];
+        above += mine[i];
+      }
+    }
+    __syncthreads();
+    prefix |= chosen[0] << shift, left = chosen[1];
+    exact = pass == 2;
+    if (chosen[2] == left) break;  // the same for all threads
   }
 
-  // ---- pages whose key is above, and the first `left` of the equals, in order
-  int above = 0, equal = 0;  // in front of this round of pages
-  for (int base = 0; base < last; base += kSelThreads) {
-    const int p = base + tid;
-    const uint32_t key = p < last ? keys[p] : 0u;
-    const unsigned is_above = __ballot_sync(0xffffffffu, p < last && want > 0 && key > prefix);
-    const unsigned is_equal = __ballot_sync(0xffffffffu, p < last && want > 0 && key == prefix);
-    if (lane == 0) warp_above[warp] = __popc(is_above), warp_equal[warp] = __popc(is_equal);
-    __syncthreads();
-    const unsigned before = (1u << lane) - 1u;
-    int my_above = above + __popc(is_above & before), my_equal = equal + __popc(is_equal & before);
-    for (int w = 0; w < kSelWarps; ++w) {
-      if (w < warp) my_above += warp_above[w], my_equal += warp_equal[w];
-      above += warp_above[w], equal += warp_equal[w];
-    }
-    const int limit = static_cast<int>(left);
-    const bool taken = (is_above >> lane & 1u) || ((is_equal >> lane & 1u) && my_equal < limit);
-    if (taken) out[my_above + (my_equal < limit ? my_equal : limit)] = p;
-    __syncthreads();
+  // ---- pages whose key is above, and the first `left` of the equals, in order: a thread has some consecutive ones
+  const int each = (last + kSelThreads - 1) / kSelThreads, begin = tid * each < last ? tid * each : last;
+  const int end = begin + each < last ? begin + each : last, limit = static_cast<int>(left);
+  auto is_above = [&](uint32_t key) { return exact ? key > prefix : key >= prefix; };
+  auto is_equal = [&](uint32_t key) { return exact && key == prefix; };
+  int above = 0, equal = 0;
+  for (int p = begin; p < end; ++p) above += is_above(keys[p]), equal += is_equal(keys[p]);
+  int above_upto = above, equal_upto = equal;
+#pragma unroll
+  for (int sh = 1; sh < 32; sh <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, above_upto, sh), w = __shfl_up_sync(0xffffffffu, equal_upto, sh);
+    if (lane >= sh) above_upto += v, equal_upto += w;
+  }
+  if (lane == 31) warp_above[warp] = above_upto, warp_equal[warp] = equal_upto;
+  __syncthreads();
+  above = above_upto - above, equal = equal_upto - equal;  // in front of this thread's pages
+  for (int w = 0; w < warp; ++w) above += warp_above[w], equal += warp_equal[w];
+  for (int p = begin; p < end; ++p) {
+    const uint32_t key = keys[p];
+    if (is_above(key) || (is_equal(key) && equal < limit)) out[above + (equal < limit ? equal : limit)] = p;
+    above += is_above(key), equal += is_equal(key);
   }
   if (tid == 0) out[want] = last;
 }
@@ -190,7 +222,7 @@ kv8_select_kernel(const __grid_constant__ SelectArgs a) {
 template <typename T>
 int dispatch_select(int64_t d, const SelectArgs& a, dim3 grid, size_t smem, cudaStream_t s) {
   auto run = [&](auto kernel) {
-    if (smem > 40 * 1024) {  // with what it has statically, beyond what a launch gets unasked
+    if (smem > 32 * 1024) {  // with the 9 KB that it has statically, beyond what a launch gets unasked
       const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
       if (err != cudaSuccess) return note_launch(err);
     }
