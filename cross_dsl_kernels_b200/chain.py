@@ -16,6 +16,9 @@ attention output and keeps the five launches data-dependent.  With
 3b. paged decode attention over the cache step 3 wrote   q_rot -> attn [tokens, hidden]
 5b. SwiGLU on the up+gate output                          upgate -> act [tokens, mlp]
 
+``kv_cache="int8"`` or ``"e4m3"`` (with ``attention=True``) holds the cache in 8 bits (kv8.py): 3 and 3b are that cache's append and
+attention, and with ``top_pages`` the attention reads only the pages of each context that score best.
+
 Multi-GPU (one process per GPU): the projections are column-sharded and the KV
 heads split, rank r owning q heads [r*Hq/g, ...), kv heads [r*Hkv/g, ...) and
 the same fraction of the up+gate columns; its QKV shard is laid out
@@ -127,7 +130,13 @@ class DecodeLayerChain:
 
     def __init__(self, cfg: ChainConfig = ChainConfig(), *, layers: int = 1, rank: int = 0, world: int = 1,
                  seed: int = 0, device="cuda", group=None, exchange: str = "peer", dependent_launch: bool = False,
-                 attention: bool = False):
+                 attention: bool = False, kv_cache: str = "f16", top_pages: int = 0):
+        if kv_cache not in ("f16", "int8", "e4m3"):
+            raise ValueError("kv_cache must be 'f16', 'int8' or 'e4m3'")
+        if kv_cache != "f16" and not attention:
+            raise ValueError("an 8-bit cache is for the layer with attention")
+        if type(top_pages) is not int or top_pages < 0 or (top_pages and kv_cache == "f16"):
+            raise ValueError("top_pages is the number of pages that the attention over an 8-bit cache reads (0: all)")
         if cfg.q_heads % world or cfg.kv_heads % world or (2 * cfg.mlp) % world:
             raise ValueError("heads and MLP columns must divide by the number of ranks")
         if exchange not in ("peer", "nccl"):
@@ -137,6 +146,7 @@ class DecodeLayerChain:
         self.cfg, self.rank, self.world, self.pg = cfg, rank, world, group
         self.exchange, self.dependent = exchange, bool(dependent_launch)
         self.attention = bool(attention)
+        self.top_pages = top_pages
         self.device = torch.device(device)
         c = cfg
         # Weights are drawn on the device (Philox, same values on every rank for one seed): drawing
@@ -174,11 +184,20 @@ class DecodeLayerChain:
         self.dev = {k: getattr(self, k).to(self.device) for k in
                     ("positions", "sequence_ids", "page_table", "cos", "sin", "h", "res")}
         shape = (pages, c.page_size, hkv, d)
-        self.k_cache = torch.full(shape, -999.0, dtype=torch.float16, device=self.device)
-        self.v_cache = torch.full(shape, -999.0, dtype=torch.float16, device=self.device)
+        self.cache8 = None
+        if kv_cache == "f16":
+            self.k_cache = torch.full(shape, -999.0, dtype=torch.float16, device=self.device)
+            self.v_cache = torch.full(shape, -999.0, dtype=torch.float16, device=self.device)
+        else:
+            from .kv8 import PagedKV8Cache
+
+            self.cache8 = PagedKV8Cache.empty(pages, c.page_size, hkv, d, dtype=torch.int8 if kv_cache == "int8" else torch.float8_e4m3fn,
+                                              means=top_pages > 0, device=self.device)
+            self.k_cache, self.v_cache = self.cache8.k, self.cache8.v
         self.arena = None
-        # a bound on the contexts from which the attention read splits the batch evenly adds its merge launch
-        merge = int(attention and _native.lib().xdk_paged_decode_attention_scratch_bytes(
+        # a bound on the contexts from which the attention read splits the batch evenly adds its merge launch; over the 8-bit cache it
+        # always has one, and the selection of pages is one more
+        merge = 1 + (top_pages > 0) if self.cache8 is not None else int(attention and _native.lib().xdk_paged_decode_attention_scratch_bytes(
             c.tokens, hq, hkv, d, c.context, _native.XDK_F16) > 0)
         if world > 1 and exchange == "peer":
             from .peer import PeerArena
@@ -206,6 +225,21 @@ class DecodeLayerChain:
         """CPU copies of one layer's unsharded weights (single-rank chains only; for checkers)."""
         return {k: v.cpu() for k, v in self.layers[layer]["full"].items()}
 
+    def _attend(self, q, peer_out=None):
+        dv, dep = self.dev, self.dependent
+        index = (dv["positions"], dv["page_table"], dv["sequence_ids"])
+        if self.cache8 is None:
+            from .ops import paged_decode_attention
+
+            return paged_decode_attention(q, self.k_cache, self.v_cache, *index, page_size=self.cfg.page_size, context_hint=self.cfg.context,
+                                          dependent_launch=dep, peer_out=peer_out)
+        from .kv8 import paged_kv8_decode_attention, paged_kv8_sparse_attention, select_kv8_pages
+
+        if self.top_pages:
+            pages = select_kv8_pages(q, self.cache8, *index, top_pages=self.top_pages, dependent_launch=dep)
+            return paged_kv8_sparse_attention(q, self.cache8, pages, *index, dependent_launch=dep, peer_out=peer_out)
+        return paged_kv8_decode_attention(q, self.cache8, *index, context_hint=self.cfg.context, dependent_launch=dep, peer_out=peer_out)
+
     def step(self, layer: int = 0, h=None, res=None) -> dict:
         """One layer: returns every intermediate (device tensors)."""
         import torch.distributed as dist
@@ -221,17 +255,19 @@ class DecodeLayerChain:
         q, k, v = qkv.view(c.tokens, hq + 2 * hkv, d).split((hq, hkv, hkv), dim=1)
         q_dst = self.q_peer[layer % 2] if peer else None
         sharded_attention = peer and self.attention
-        q_rot = rope_gqa_paged_kv_append(q, k, v, dv["cos"], dv["sin"], dv["positions"], dv["page_table"],
-                                         dv["sequence_ids"], self.k_cache, self.v_cache, page_size=c.page_size,
-                                         rope_dim=d, interleaved=False, kv_layout="NHD", dependent_launch=dep,
-                                         q_peer_out=q_dst.out_for(self.rank * hq * d) if peer and not sharded_attention else None)
-        if sharded_attention:
-            from .ops import paged_decode_attention
+        if self.cache8 is not None:
+            from .kv8 import rope_gqa_paged_kv8_append
 
+            q_rot = rope_gqa_paged_kv8_append(q, k, v, dv["cos"], dv["sin"], dv["positions"], dv["page_table"], dv["sequence_ids"],
+                                              self.cache8, rope_dim=d, interleaved=False, dependent_launch=dep)
+        else:
+            q_rot = rope_gqa_paged_kv_append(q, k, v, dv["cos"], dv["sin"], dv["positions"], dv["page_table"],
+                                             dv["sequence_ids"], self.k_cache, self.v_cache, page_size=c.page_size,
+                                             rope_dim=d, interleaved=False, kv_layout="NHD", dependent_launch=dep,
+                                             q_peer_out=q_dst.out_for(self.rank * hq * d) if peer and not sharded_attention else None)
+        if sharded_attention:
             # this rank's heads against its own cache shard; every rank receives the result
-            paged_decode_attention(q_rot, self.k_cache, self.v_cache, dv["positions"], dv["page_table"], dv["sequence_ids"],
-                                   page_size=c.page_size, context_hint=c.context, dependent_launch=dep,
-                                   peer_out=q_dst.out_for(self.rank * hq * d))
+            self._attend(q_rot, peer_out=q_dst.out_for(self.rank * hq * d))
             self.arena.barrier(self.site_q, dependent_launch=dep)
             attn = q_dst.local
         elif peer:
@@ -241,10 +277,7 @@ class DecodeLayerChain:
             dist.all_gather_into_tensor(self.q_gather, q_rot.view(c.tokens, hq * d), group=self.pg)
             attn = unshard_columns(self.q_gather, self.q_full)
         elif self.attention:
-            from .ops import paged_decode_attention
-
-            attn = paged_decode_attention(q_rot, self.k_cache, self.v_cache, dv["positions"], dv["page_table"], dv["sequence_ids"],
-                                          page_size=c.page_size, context_hint=c.context, dependent_launch=dep).view(c.tokens, c.hidden)
+            attn = self._attend(q_rot).view(c.tokens, c.hidden)
         else:
             attn = q_rot.view(c.tokens, c.hidden)
         n2, r2 = fused_residual_rmsnorm(attn, r1, L["w2"], c.eps, dependent_launch=dep)

@@ -73,6 +73,10 @@ __device__ __forceinline__ float exp2_fast(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ void prefetch_l1(const void* p) {  // a load that nobody waits for
+  uint16_t unused;
+  asm volatile("ld.global.u16 %0, [%1];" : "=h"(unused) : "l"(p));
+}
 __device__ __forceinline__ float log2_fast(float x) {
   float y;
   asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -147,6 +151,9 @@ template <bool SPARSE> __device__ __forceinline__ int tiles_of(const Kv8Args& a,
 template <bool SPARSE> __device__ __forceinline__ int units_of(const Kv8Args& a, int token) {  // of one of its heads
   return token < a.tokens ? tiles_of<SPARSE>(a, a.positions[token] + 1) + kEntry : 0;
 }
+__device__ __forceinline__ int64_t divide(int64_t x, int64_t y) {  // of what is not below 0; in 32 bits where they do
+  return ((x | y) >> 31) == 0 ? static_cast<uint32_t>(x) / static_cast<uint32_t>(y) : x / y;
+}
 // Whole warps call these.
 template <bool SPARSE> __device__ __forceinline__ int64_t count_units(const Kv8Args& a) {
   int64_t total = 0;
@@ -174,7 +181,7 @@ template <bool SPARSE> __device__ __forceinline__ Cursor find_unit(const Kv8Args
       const int src = __ffs(who) - 1, each = __shfl_sync(0xffffffffu, units, src);
       const int64_t at = from - before - __shfl_sync(0xffffffffu, upto - mine, src);
       c.token = t0 + src, c.tiles = each - kEntry;
-      c.kvh = static_cast<int>(at / each);
+      c.kvh = static_cast<int>(divide(at, each));
       const int in = static_cast<int>(at - static_cast<int64_t>(c.kvh) * each) - kEntry;
       c.tile = in > 0 ? in : 0;
       c.left = to - from + (in < 0 ? in : 0);
@@ -231,10 +238,11 @@ kv8_attention_kernel(const __grid_constant__ Kv8Args a, const __grid_constant__ 
   const int lane = threadIdx.x;
   const int grow = lane >> 2, quad = lane & 3;
   const int G = a.group;
+  if (lane < a.tokens) prefetch_l1(a.sequence_ids + lane);  // needed once the token is known
   const int64_t total = count_units<SPARSE>(a), warps = total < gridDim.x ? total : gridDim.x;
   if (blockIdx.x >= warps) return;
-  const int64_t end_unit = total * (blockIdx.x + 1) / warps;
-  Cursor cur = find_unit<SPARSE>(a, total * blockIdx.x / warps, end_unit);  // the tile that is computed next
+  const int64_t end_unit = divide(total * (blockIdx.x + 1), warps);
+  Cursor cur = find_unit<SPARSE>(a, divide(total * blockIdx.x, warps), end_unit);  // the tile that is computed next
   if (cur.left == 0) return;
   Cursor next = cur;  // the tile that is fetched next, and what its rows are found by
   int64_t ctx = 0, coming_ctx = 0, coming_seq = 0;  // of the token, and of the one behind it
@@ -252,10 +260,7 @@ kv8_attention_kernel(const __grid_constant__ Kv8Args a, const __grid_constant__ 
     // q of the item, which is loaded when its first tile is computed, on its way to L1
     const int bytes = G * D * (SPLIT ? 4 : 2);
     const unsigned char* at = static_cast<const unsigned char*>(a.q) + (static_cast<int64_t>(next.token) * a.q_heads + next.kvh * G) * (D * (SPLIT ? 4 : 2));
-    for (int i = lane * 128; i < bytes; i += 32 * 128) {
-      uint16_t unused;
-      asm volatile("ld.global.u16 %0, [%1];" : "=h"(unused) : "l"(at + i));
-    }
+    for (int i = lane * 128; i < bytes; i += 32 * 128) prefetch_l1(at + i);
   };
   int64_t page[R];  // of this lane's rows of it, -1: dead
   int off[R];

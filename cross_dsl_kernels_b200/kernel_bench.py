@@ -5,7 +5,7 @@ rotate over enough distinct buffer sets to defeat the L2 (see timing.py),
 replayed and event-timed; ``gbps`` is the op's algorithmic bytes over the
 per-call median.  Used by bench.py and usable on its own:
 
-    python -m cross_dsl_kernels_b200.kernel_bench [rmsnorm|gemv|rope|w4a16] ...
+    python -m cross_dsl_kernels_b200.kernel_bench [rmsnorm|gemv|rope|w4a16|kv8] ...
 
 Every ``bench_*`` function takes an optional ``check(stage, outputs)``: the
 caller's gate, run on the eager result, on a replay with poisoned outputs and
@@ -166,6 +166,51 @@ def bench_attention(context: int, tokens: int = 16, q_heads: int = 32, kv_heads:
     return _row(name + ("_pdl" if dependent else ""), nbytes, t, sets, peak)
 
 
+def bench_kv8(op: str, context: int, tokens: int = 16, codes=torch.int8, top_pages: int = 64, q_heads: int = 32, kv_heads: int = 8,
+              head_dim: int = 128, page_size: int = 16, dtype=torch.float16, peak=None, replays=20, check=None, dependent=False) -> dict:
+    """One op of the 8-bit cache -- ``op``: "append" (one token per sequence), "attention", "select" or "sparse" (over the pages that
+    "select" chose) -- on ``tokens`` sequences, each ``context`` positions long."""
+    from . import kv8
+
+    per_seq = -(-context // page_size)
+    rows, row, ends = tokens * kv_heads, head_dim, 2 * tokens * q_heads * head_dim * dtype.itemsize
+    top = min(top_pages, per_seq)
+    nbytes = {"append": wl.rope_bytes(tokens, q_heads, kv_heads, head_dim, head_dim, dtype) - 2 * rows * row * (dtype.itemsize - 1),
+              "attention": rows * (2 * context * row + 8 * per_seq) + ends, "select": rows * per_seq * (row + 4) + ends // 2 + 4 * rows * top,
+              "sparse": rows * top * (2 * page_size * row + 8 + 4) + ends}[op]
+    sets = rotation_for(nbytes, cap=16)
+    g = torch.Generator(device="cuda").manual_seed(context)
+    cache = kv8.PagedKV8Cache.empty(sets * tokens * per_seq, page_size, kv_heads, head_dim, dtype=codes)
+    for t in (cache.k, cache.v):  # codes of any value but those of e4m3 that are none
+        t.view(torch.uint8).copy_(torch.randint(0, 0x7f, t.shape, generator=g, device="cuda", dtype=torch.uint8))
+    for t in (cache.k_scale, cache.v_scale):
+        t.uniform_(0.005, 0.02, generator=g)
+    cache.k_mean.copy_(torch.randint(-60, 61, cache.k_mean.shape, generator=g, device="cuda", dtype=torch.int8))
+    order = torch.randperm(cache.pages, generator=torch.Generator().manual_seed(context)).reshape(sets, tokens, per_seq).cuda()
+    tables = [order[i].contiguous() for i in range(sets)]
+    positions, ids = torch.full((tokens,), context - 1, dtype=torch.int64, device="cuda"), torch.arange(tokens, device="cuda")
+    q, k, v = (torch.randn(tokens, h, head_dim, generator=g, device="cuda", dtype=dtype) for h in (q_heads, kv_heads, kv_heads))
+    angle = torch.rand(context, head_dim // 2, generator=g, device="cuda")
+    cos, sin = angle.cos(), angle.sin()
+
+    def run(i):
+        index, kw = (positions, tables[i % sets], ids), dict(dependent_launch=dependent)
+        if op == "append":
+            return kv8.rope_gqa_paged_kv8_append(q, k, v, cos, sin, *index, cache, rope_dim=head_dim, interleaved=False, **kw)
+        if op == "attention":
+            return kv8.paged_kv8_decode_attention(q, cache, *index, context_hint=context, **kw)
+        if op == "select":
+            return kv8.select_kv8_pages(q, cache, *index, top_pages=top, **kw)
+        return kv8.paged_kv8_sparse_attention(q, cache, chosen[i % sets], *index, **kw)
+
+    chosen = [kv8.select_kv8_pages(q, cache, positions, tables[i], ids, top_pages=top) for i in range(sets)] if op == "sparse" else []
+    calls = [(lambda i=i: (run(i), q, cache, positions, tables[i % sets], ids)) for i in range(_calls_per_graph(sets))]
+    t = graph_median_us(calls, replays, check=check, mutate=lambda: q.neg_(),
+                        poison=lambda outs: [o[0].fill_(float("nan") if o[0].is_floating_point() else -1) for o in outs])
+    name = f"kv8_{op}_{str(codes).split('.')[-1]}_t{tokens}_hq{q_heads}_hkv{kv_heads}_d{head_dim}_ctx{context}"
+    return _row(name + (f"_top{top}" if op in ("select", "sparse") else "") + ("_pdl" if dependent else ""), nbytes, t, sets, peak)
+
+
 def bench_swiglu(rows: int, width: int, dtype=torch.float16, peak=None, replays=20, check=None, dependent=False) -> dict:
     nbytes = 3 * rows * width * dtype.itemsize
     sets = rotation_for(nbytes, cap=48)
@@ -246,6 +291,11 @@ def table(which=("rmsnorm", "gemv", "rope", "w4a16"), peak=None, split_sweep=Tru
         for n in (4096, 14336):
             for m in (1, 16):
                 rows.append(bench_w4a16(m, 4096, n, 128, peak))
+    if "kv8" in which:
+        for codes in (torch.int8, torch.float8_e4m3fn):
+            for op in ("append", "attention", "select", "sparse"):
+                for tokens in (1, 16):
+                    rows.append(bench_kv8(op, 8192, tokens, codes, peak=peak))
     if "chain" in which:
         rows.append(bench_chain(peak=peak))
     return rows
@@ -254,7 +304,7 @@ def table(which=("rmsnorm", "gemv", "rope", "w4a16"), peak=None, split_sweep=Tru
 def one(argv: list[str]) -> dict:
     """``--one rmsnorm ROWS HIDDEN f32|bf16|f16`` | ``--one gemv M K N KN|NK SPLIT [strict]`` |
     ``--one rope f32|bf16 NHD|HND ROPE_DIM`` | ``--one w4a16 M K N GROUP`` | ``--one attention CONTEXT [TOKENS]`` |
-    ``--one swiglu ROWS WIDTH``; few replays (for profilers)."""
+    ``--one swiglu ROWS WIDTH`` | ``--one kv8 append|attention|select|sparse CONTEXT [TOKENS]``; few replays (for profilers)."""
     dtypes = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
     op, rest = argv[0], argv[1:]
     if op == "rmsnorm":
@@ -270,6 +320,8 @@ def one(argv: list[str]) -> dict:
         return bench_attention(int(rest[0]), tokens=int(rest[1]) if len(rest) > 1 else 16, replays=3)
     if op == "swiglu":
         return bench_swiglu(int(rest[0]), int(rest[1]), replays=3)
+    if op == "kv8":
+        return bench_kv8(rest[0], int(rest[1]), int(rest[2]) if len(rest) > 2 else 16, replays=3)
     raise SystemExit(one.__doc__)
 
 
