@@ -7,10 +7,13 @@
 // the same whatever computes it.  One choice per token and KV head: the query heads that share it read its pages together.
 //
 // One CTA per (token, KV head).  Scores: mma.m16n8k32 on bytes, 16 pages as rows, the heads of the group as columns; a thread
-// loads a quarter of two pages' means with 16-byte loads, those of a few blocks of pages at a time, and the codes of q stand in
-// registers in the same order of dims.  The scores stay in shared memory as sortable integers; up to three passes over 11, 11 and 10 bits of
-// them find the value of the last one chosen (two, mostly: no other has its first 22 bits), one more writes the pages in order.
-// Bound: short contexts by the chain of loads and barriers, long ones by the latency of the reads of the means.
+// loads a quarter of two pages' means with 16-byte loads, four threads 64 bytes in a row (14.0 us for 16 tokens, 8 KV heads and
+// 2048 pages; a quarter of the dims in a row to each thread: 14.5), those of four blocks of 16 pages at a time (the next four loaded
+// during these ones' products: 14.7), and the codes of q stand in registers in the same order of dims.  The scores stay in shared
+// memory as sortable integers; up to three passes over 11, 11 and 10 bits of them find the value of the last one chosen (two, mostly:
+// no other has its first 22 bits), one more writes the pages in order.
+// Bound: 512 pages (7.3 us for one token) by the chain of loads and barriers; 2048 pages, whose means are 35 MB, by the latency of
+// their reads: 2.3 us in front of the scores, 8.4 for them, 3.3 for the choice.
 #include <math.h>
 
 #include "kv8.cuh"
@@ -103,9 +106,9 @@ kv8_select_kernel(const __grid_constant__ SelectArgs a) {
 
   // ---- scores
   const int row = lane >> 2, quad = lane & 3;
-  uint32_t b[kWords];  // head `row`, dims quad * D / 4 ..
+  uint32_t b[kWords];  // head `row`, dims 64 i + 16 quad .. + 15
 #pragma unroll
-  for (int w = 0; w < kWords; ++w) b[w] = codes[row][quad * kWords + w];
+  for (int w = 0; w < kWords; ++w) b[w] = codes[row][w / 4 * 16 + quad * 4 + w % 4];
   const float unit0 = unit[2 * quad], unit1 = unit[2 * quad + 1];
   const bool live0 = 2 * quad < group, live1 = 2 * quad + 1 < group;
   constexpr int kAtOnce = D <= 128 ? 4 : 2;  // blocks of 16 pages whose loads are on their way together
@@ -127,7 +130,7 @@ kv8_select_kernel(const __grid_constant__ SelectArgs a) {
         if (base0 + u * kSelWarps * 16 >= last) continue;
 #pragma unroll
         for (int w = 0; w < kWords; w += 4) {
-          const U4 v = ld_ordered_stream16(a.k_mean + block[u][r] * D + quad * (D / 4) + w * 4);
+          const U4 v = ld_ordered_stream16(a.k_mean + block[u][r] * D + w * 16 + quad * 16);
           m[u][r][w] = v.x, m[u][r][w + 1] = v.y, m[u][r][w + 2] = v.z, m[u][r][w + 3] = v.w;
         }
         scale[u][r] = a.k_scale[block[u][r]];
