@@ -272,7 +272,7 @@ __device__ __forceinline__ void divide16(const Divider& d, float (&x)[16]) {
   for (int e = 0; e < 16; ++e) {
     float q = __fmul_rn(x[e], d.r);
     q = __fmaf_rn(__fmaf_rn(-q, d.scale, x[e]), d.r, q);
-    x[e] = __fmaf_rn(__fmaf_rn(-q, d.scale, x[e]), d.r, q);
+    x[e] = copysignf(__fmaf_rn(__fmaf_rn(-q, d.scale, x[e]), d.r, q), x[e]);  // -0 too, which e4m3 has
   }
 }
 
@@ -566,7 +566,7 @@ extern "C" int xdk_kv8_append(const void* q, const void* k, const void* v, const
   if (tokens < 1 || q_heads < 1 || kv_heads < 1 || head_dim < 1 || page_size < 1 || max_pages_per_seq < 1) return XDK_ERR_ARG;
   if (q_heads % kv_heads != 0 || rope_dim < 2 || rope_dim % 2 != 0 || rope_dim > head_dim || cos_width < rope_dim / 2) return XDK_ERR_ARG;
   if (q_token_stride < q_heads * head_dim || k_token_stride < kv_heads * head_dim || v_token_stride < kv_heads * head_dim) return XDK_ERR_ARG;
-  if (!aligned16(q_out) || !aligned16(k_cache) || !aligned16(v_cache)) return XDK_ERR_ARG;
+  if (!aligned16(q_out) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(k_mean)) return XDK_ERR_ARG;
   if (!kv8_head_dim(head_dim) || q_heads > 65535 || cos_width > 2147483647LL) return XDK_ERR_LIMIT;
   if (int st = kv8_limits(tokens, kv_heads, max_pages_per_seq, page_size)) return st;
   const size_t need = xdk_kv8_append_scratch_bytes(tokens, kv_heads);

@@ -164,6 +164,63 @@ def test_append_takes_slices_of_a_fused_projection_and_wide_tables():
     _same(ours, cache)
 
 
+@pytest.mark.parametrize("codes", [INT8, E4M3])
+@pytest.mark.parametrize("tokens", [100, 900])
+def test_append_quotients(codes, tokens):
+    """Quotients on and next to the middle between two codes, for scales from the smallest subnormal to beyond the middle of the
+    exponents' range, with significands of all ones among them: the bytes of a division that is rounded once."""
+    g, dim, top = _gen(tokens), 256, oracle.TOP[codes]
+    most = torch.ldexp(1 + torch.rand(tokens, generator=g), torch.linspace(-149, 126, tokens).round().int())
+    most[::7] = torch.ldexp(torch.full_like(most, 2 - 2.0 ** -23), torch.linspace(-149, 126, tokens).round().int())[::7]
+    scale = most * (torch.tensor(1.0) / top)
+    every = torch.arange(256, dtype=torch.uint8).view(codes).double()
+    every = every[every.isfinite()].sort().values
+    middle = ((every[1:] + every[:-1]) / 2)[torch.randint(0, every.numel() - 1, (tokens, dim), generator=g)]
+    x = (middle * scale.double()[:, None]).float()
+    step = torch.randint(-1, 2, x.shape, generator=g)
+    x = torch.where(step == 0, x, torch.nextafter(x, step * torch.inf))
+    x = x.clamp(-most[:, None], most[:, None])
+    x[:, 0] = most
+    cache, pos = oracle.empty(tokens, 1, 1, dim, codes), torch.zeros(tokens, dtype=torch.int64)
+    _append(_on_gpu(cache, "NHD"), cache, *(t[:, None].contiguous() for t in (x, x, -x)), _trig(1, dim), pos, _table(tokens, 1, 1),
+            torch.arange(tokens), rope_dim=dim, interleaved=False)
+
+
+@pytest.mark.parametrize("tokens", [128, 300])
+def test_append_without_means_captured_twice(tokens):
+    """Two graphs of one stream, each a prompt's append with what it needs besides, replayed in turn on changed inputs; no mean keys."""
+    from dataclasses import replace
+    from cross_dsl_kernels_b200.kv8 import rope_gqa_paged_kv8_append
+    g, dim, page = _gen(tokens), 64, 16
+    trig, pos, seq = _trig(512, dim), torch.arange(tokens) % 150, torch.arange(tokens) // 150
+    table = _table(3, 10, 5)
+    caches = [_filled(30, page, 2, dim, codes, 6) for codes in (INT8, E4M3)]
+    ours = [replace(_on_gpu(cache, "HND"), k_mean=None) for cache in caches]
+    inputs = [torch.zeros(tokens, h, dim, dtype=BF16, device="cuda") for h in (4, 2, 2)]
+    index, dev = [pos.cuda(), table.cuda(), seq.cuda()], [t.cuda() for t in trig]
+    stream, graphs, outs = torch.cuda.Stream(), [], []
+    with torch.cuda.stream(stream):
+        for cache in ours:
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=stream):
+                outs.append(rope_gqa_paged_kv8_append(*inputs, *dev, *index, cache, rope_dim=dim, interleaved=True, dependent_launch=True))
+            graphs.append(graph)
+    torch.cuda.synchronize()
+    for _ in range(3):
+        fresh = [_values(tokens, h, dim, BF16, g) for h in (4, 2, 2)]
+        for to, x in zip(inputs, fresh):
+            to.copy_(x)
+        for graph in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for cache, own, out in zip(caches, ours, outs):
+            means = cache["k_mean"].clone()
+            want = oracle.append(*fresh, *trig, pos, table, seq, cache, rope_dim=dim, interleaved=True)
+            cache["k_mean"] = means  # the restatement always keeps them
+            assert torch.equal(out.cpu(), want)
+            _same(replace(own, k_mean=means.cuda()), cache)
+
+
 # ---- attention -------------------------------------------------------------------------------------------------------------
 
 
@@ -284,6 +341,39 @@ def test_attention_far_into_a_large_cache():
         assert torch.equal(getattr(ours, name)[-4:].cpu(), small[name]), name
 
 
+@pytest.mark.parametrize("tokens,heads", [(65535, (2, 1)), (2500, (9, 3))])
+def test_many_tokens(tokens, heads):
+    """The most tokens a call takes, of few sequences over and over, for all three ops that read the cache."""
+    from cross_dsl_kernels_b200 import kv8
+    dim, page, few = 64, 8, 61
+    cache, pos, table, seq = _attend_inputs(heads, dim, page, [(i * 37) % 100 - 1 for i in range(few)], INT8, seed=17)
+    q = torch.randn(few, heads[0], dim, generator=_gen(17)).half()
+    of, ours = torch.arange(tokens) % few, _on_gpu(cache, "NHD")
+    args = [pos[of].cuda(), table.cuda(), seq[of].cuda()]
+    many = lambda exact: {name: x[of] for name, x in exact.items()}  # noqa: E731
+    chosen = oracle.select(q, cache, pos, table, seq, top_pages=4)
+    assert torch.equal(kv8.select_kv8_pages(q[of].cuda(), ours, *args, top_pages=4).cpu(), chosen[of])
+    whole, some = oracle.attention(q, cache, pos, table, seq), oracle.attention(q, cache, pos, table, seq, pages=chosen)
+    for hint in (0, 100):
+        _close(kv8.paged_kv8_decode_attention(q[of].cuda(), ours, *args, context_hint=hint), many(whole), F16, dim)
+    _close(kv8.paged_kv8_sparse_attention(q[of].cuda(), ours, chosen[of].cuda(), *args), many(some), F16, dim)
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+def test_q_that_begins_anywhere(dtype):
+    """A contiguous q whose first element is not on a 16-byte boundary: the same bits as one on it."""
+    from cross_dsl_kernels_b200 import kv8
+    cache, pos, table, seq = _attend_inputs((8, 2), 128, 16, [700, 3, -1], E4M3, seed=18)
+    q = torch.randn(3, 8, 128, generator=_gen(18)).to(dtype).cuda()
+    shifted = torch.empty(q.numel() + 1, dtype=dtype, device="cuda")[1:].view_as(q)
+    shifted.copy_(q)
+    ours, args = _on_gpu(cache, "HND"), [t.cuda() for t in (pos, table, seq)]
+    pages = kv8.select_kv8_pages(q, ours, *args, top_pages=5)
+    assert torch.equal(pages, kv8.select_kv8_pages(shifted, ours, *args, top_pages=5))
+    assert torch.equal(kv8.paged_kv8_decode_attention(q, ours, *args), kv8.paged_kv8_decode_attention(shifted, ours, *args))
+    assert torch.equal(kv8.paged_kv8_sparse_attention(q, ours, pages, *args), kv8.paged_kv8_sparse_attention(shifted, ours, pages, *args))
+
+
 # ---- selection and the attention over the selected pages -----------------------------------------------------------------------
 
 
@@ -317,6 +407,20 @@ def test_selection_of_equals_and_of_not_a_number():
     cache["k_scale"][at[1234]] = float("nan")
     got = select_kv8_pages(-q.cuda(), _on_gpu(cache, "NHD"), *(t.cuda() for t in (pos, table, seq)), top_pages=3).cpu()
     assert got.flatten().tolist() == [0, 1234, 1500]
+
+
+@pytest.mark.parametrize("value", [float("inf"), float("-inf"), float("nan")])
+def test_selection_by_a_q_that_is_not_finite(value):
+    """No choice is better than another then; each is still one of pages of the context, ascending, the last one among them."""
+    from cross_dsl_kernels_b200.kv8 import select_kv8_pages
+    cache, pos, table, seq = _attend_inputs((4, 2), 64, 4, [1000, 399, 7], INT8, seed=19)
+    q = torch.randn(3, 4, 64, generator=_gen(19))
+    q[:, 1, 5] = value
+    got = select_kv8_pages(q.cuda(), _on_gpu(cache, "NHD"), *(t.cuda() for t in (pos, table, seq)), top_pages=9).cpu()
+    assert torch.equal(got[:, 1], oracle.select(q, cache, pos, table, seq, top_pages=9)[:, 1])  # the head that has numbers
+    for t, last in ((0, 250), (1, 99)):
+        assert (got[t].diff() > 0).all() and (got[t, :, 0] >= 0).all() and (got[t, :, -1] == last).all()
+    assert got[2].tolist() == [[0, 1] + [-1] * 7] * 2
 
 
 @pytest.mark.parametrize("codes", [INT8, E4M3])
@@ -432,3 +536,39 @@ def test_streams_and_a_wider_destination():
     assert torch.equal(wide[:, 40:552], want[0].view(2, 512)) and (wide[:, :40] == -7).all() and (wide[:, 552:] == -7).all()
     kv8.paged_kv8_sparse_attention(q, ours, pages, *args, peer_out=dst)
     assert torch.equal(wide[:, 40:552], want[1].view(2, 512))
+
+
+def test_two_streams_at_once():
+    """Steps over two caches on two streams, whose kernels run side by side: what each gives alone."""
+    heads, dim, page, top = (8, 2), 64, 16, 12
+    g, trig = _gen(20), [t.cuda() for t in _trig(4096, dim)]
+    sides = []
+    for codes in (INT8, E4M3):
+        cache, pos, table, seq = _attend_inputs(heads, dim, page, [4000, 31, 2222, 800], codes, seed=20)
+        qkv = [torch.randn(4, h, dim, generator=g).half().cuda() for h in (8, 2, 2)]
+        many = [torch.randn(300, h, dim, generator=g).half().cuda() for h in (8, 2, 2)]
+        sides.append((cache, qkv, many, [t.cuda() for t in (pos, table, seq)]))
+
+    def run(side, ours):
+        from cross_dsl_kernels_b200.kv8 import rope_gqa_paged_kv8_append
+        cache, qkv, many, (pos, table, seq) = side
+        at, of = torch.arange(300, device="cuda") % 75, torch.arange(300, device="cuda") // 75
+        got = []
+        for step in range(6):
+            got += _step(ours, *qkv, trig, pos + step, table, seq, top)
+            got.append(rope_gqa_paged_kv8_append(*many, *trig, at + step, table, of, ours, rope_dim=dim, interleaved=False))
+        return got
+
+    alone = []
+    for side in sides:
+        alone.append(run(side, _on_gpu(side[0], "NHD")))
+        torch.cuda.synchronize()
+    streams, again, got = [torch.cuda.Stream() for _ in sides], [_on_gpu(side[0], "NHD") for side in sides], []
+    torch.cuda.synchronize()
+    for side, stream, ours in zip(sides, streams, again):
+        with torch.cuda.stream(stream):
+            torch.cuda._sleep(5_000_000)
+            got.append(run(side, ours))
+    torch.cuda.synchronize()
+    for a, b in zip(alone, got):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))

@@ -87,9 +87,9 @@ def test_c_entry_points_check_sizes_before_they_touch_a_gpu():
         s = {**good, **kw}
         return lib.xdk_kv8_select_pages(p, mean, p, p, p, p, p, s["tokens"], s["hq"], s["hkv"], s["dim"], s["width"], s["page"], top, 0, 0, None)
 
-    def append(cache=p, rope=64, cw=32, qs=256, codes=0, dtype=0, scratch=None, nbytes=0, flags=0, **kw):
+    def append(cache=p, mean=None, rope=64, cw=32, qs=256, codes=0, dtype=0, scratch=None, nbytes=0, flags=0, **kw):
         s = {**good, **kw}
-        return lib.xdk_kv8_append(p, p, p, p, p, p, p, p, p, cache, p, p, p, None, s["tokens"], s["hq"], s["hkv"], s["dim"], cw, s["width"], s["page"],
+        return lib.xdk_kv8_append(p, p, p, p, p, p, p, p, p, cache, p, p, p, mean, s["tokens"], s["hq"], s["hkv"], s["dim"], cw, s["width"], s["page"],
                                   rope, qs, 128, 128, 0, 0, dtype, codes, scratch, nbytes, flags, None)
 
     wrong, limit = -1, -4
@@ -104,7 +104,7 @@ def test_c_entry_points_check_sizes_before_they_touch_a_gpu():
     dst.ld = 4 * 64
     assert sparse() == wrong and sparse(scratch=p, nbytes=64) == wrong and sparse(n=0) == wrong and sparse(pages=None) == wrong and sparse(n=1 << 22) == limit
     assert select(top=0) == wrong and select(mean=None) == wrong and select(mean=p + 4) == wrong and select(width=51201) == limit and select(hq=18) == limit
-    for kw in (dict(cache=None), dict(cache=p + 1), dict(rope=3), dict(rope=66), dict(rope=0), dict(cw=31), dict(qs=255), dict(codes=2),
+    for kw in (dict(cache=None), dict(cache=p + 1), dict(mean=p + 4), dict(rope=3), dict(rope=66), dict(rope=0), dict(cw=31), dict(qs=255), dict(codes=2),
                dict(dtype=7), dict(flags=1), dict(tokens=129), dict(tokens=129, scratch=p, nbytes=64), dict(tokens=-1)):
         assert append(**kw) == wrong, kw
     for kw in (dict(dim=192, qs=768), dict(page=2000), dict(tokens=(1 << 26) + 1)):
