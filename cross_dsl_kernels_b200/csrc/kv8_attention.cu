@@ -25,6 +25,8 @@
 // for 16 contexts of 8192; a chunk's start costs its warp 6 us without loads.)
 #include <math.h>
 
+#include <type_traits>
+
 #include "kv8.cuh"
 #include "mma_f16.cuh"
 
@@ -43,6 +45,8 @@ struct Kv8Args {
   int n_pages, dtype;                    // dtype: of q and out
   int tile;                              // positions of a tile
   int hnd, narrow;                       // narrow: every position that a page table row can hold fits 31 bits
+  int by_warp;                           // see Partials
+  int paired;                            // two dims of the output are one store
   float scale;
 };
 
@@ -124,6 +128,30 @@ __device__ __forceinline__ void store_from_f32(const PeerOut& out, int64_t row, 
   else if (dtype == XDK_BF16) peer_store(out, row, col, __float2bfloat16_rn(v));
   else peer_store(out, row, col, __float2half_rn(v));
 }
+// Dims 16 c and 16 c + 1 behind `col` of one row, c < N: value(c, 0) and value(c, 1).  `paired`: both in one store, everywhere.
+template <bool WIDE, typename Value, typename N>
+__device__ __forceinline__ void store_dims(const PeerOut& out, int64_t row, int64_t col, int dtype, bool paired, Value value, N) {
+  const int64_t at = row * out.ld + out.col0 + col;
+#pragma unroll 1
+  for (int p = 0; p < out.world; ++p) {
+    if constexpr (WIDE) {
+      float* to = static_cast<float*>(out.ptr[p]) + at;
+#pragma unroll
+      for (int c = 0; c < N::value; ++c) {
+        if (paired) *reinterpret_cast<float2*>(to + c * 16) = make_float2(value(c, 0), value(c, 1));
+        else to[c * 16] = value(c, 0), to[c * 16 + 1] = value(c, 1);
+      }
+    } else {
+      uint16_t* to = static_cast<uint16_t*>(out.ptr[p]) + at;
+#pragma unroll
+      for (int c = 0; c < N::value; ++c) {
+        const uint32_t both = dtype == XDK_BF16 ? Mma16816<__nv_bfloat16>::pack(value(c, 0), value(c, 1)) : Mma16816<__half>::pack(value(c, 0), value(c, 1));
+        if (paired) *reinterpret_cast<uint32_t*>(to + c * 16) = both;
+        else to[c * 16] = static_cast<uint16_t>(both), to[c * 16 + 1] = static_cast<uint16_t>(both >> 16);
+      }
+    }
+  }
+}
 // Statistics in units of log2: merges (m, l) of b into a.
 __device__ __forceinline__ void merge_stats2(float& m_a, float& l_a, float& scale_a, float& scale_b, float m_b, float l_b) {
   const float m = fmaxf(m_a, m_b);
@@ -155,41 +183,79 @@ __device__ __forceinline__ int64_t divide(int64_t x, int64_t y) {  // of what is
   return ((x | y) >> 31) == 0 ? static_cast<uint32_t>(x) / static_cast<uint32_t>(y) : x / y;
 }
 // Whole warps call these.
-template <bool SPARSE> __device__ __forceinline__ int64_t count_units(const Kv8Args& a) {
-  int64_t total = 0;
-  for (int t = threadIdx.x; t < a.tokens; t += 32) total += units_of<SPARSE>(a, t);
+__device__ __forceinline__ int64_t sum_upto(int64_t x) {  // over the lanes up to this one
 #pragma unroll
-  for (int sh = 16; sh > 0; sh >>= 1) total += __shfl_xor_sync(0xffffffffu, total, sh);
-  return total * a.kv_heads;
+  for (int sh = 1; sh < 32; sh <<= 1) {
+    const int64_t v = __shfl_up_sync(0xffffffffu, x, sh);
+    if (static_cast<int>(threadIdx.x) >= sh) x += v;
+  }
+  return x;
+}
+// The units of the line; of the first 32 tokens lane t knows those of a head of token t, and of all heads of the tokens up to it.
+struct Line {
+  int units;
+  int64_t upto, total;
+};
+template <bool SPARSE> __device__ __forceinline__ Line count_units(const Kv8Args& a) {
+  Line l;
+  l.units = units_of<SPARSE>(a, threadIdx.x);
+  l.upto = sum_upto(static_cast<int64_t>(l.units) * a.kv_heads);
+  l.total = __shfl_sync(0xffffffffu, l.upto, 31);
+  if (a.tokens > 32) {
+    int64_t further = 0;
+#pragma unroll 4
+    for (int t = threadIdx.x + 32; t < a.tokens; t += 32) further += units_of<SPARSE>(a, t);
+#pragma unroll
+    for (int sh = 16; sh > 0; sh >>= 1) further += __shfl_xor_sync(0xffffffffu, further, sh);
+    l.total += further * a.kv_heads;
+  }
+  return l;
 }
 // The first tile among units [from, to), whose `left` is 0 if there is none.
-template <bool SPARSE> __device__ __forceinline__ Cursor find_unit(const Kv8Args& a, int64_t from, int64_t to) {
+template <bool SPARSE> __device__ __forceinline__ Cursor find_unit(const Kv8Args& a, const Line& line, int64_t from, int64_t to) {
+  constexpr int kEach = 4;  // tokens of a lane at a time, behind the first 32 (one: 4096 tokens of 32 positions 19 us more)
   const int lane = threadIdx.x;
   Cursor c = {};
-  int64_t before = 0;
-  for (int t0 = 0; t0 < a.tokens; t0 += 32) {
-    const int units = units_of<SPARSE>(a, t0 + lane);
-    const int64_t mine = static_cast<int64_t>(units) * a.kv_heads;
-    int64_t upto = mine;
+  int64_t at = from;  // of the units from token c.token on
+  int each = 0;       // units of a head of that
+  unsigned who = __ballot_sync(0xffffffffu, from < line.upto);
+  if (who != 0) {
+    c.token = __ffs(who) - 1;
+    each = __shfl_sync(0xffffffffu, line.units, c.token);
+    at -= __shfl_sync(0xffffffffu, line.upto, c.token) - static_cast<int64_t>(each) * a.kv_heads;
+  } else {
+    at -= __shfl_sync(0xffffffffu, line.upto, 31);
+    for (int t0 = 32; t0 < a.tokens; t0 += 32 * kEach) {
+      int units[kEach];
+      int64_t mine = 0;
 #pragma unroll
-    for (int sh = 1; sh < 32; sh <<= 1) {
-      const int64_t v = __shfl_up_sync(0xffffffffu, upto, sh);
-      if (lane >= sh) upto += v;
+      for (int i = 0; i < kEach; ++i) units[i] = units_of<SPARSE>(a, t0 + lane * kEach + i), mine += units[i];
+      mine *= a.kv_heads;
+      const int64_t upto = sum_upto(mine);
+      who = __ballot_sync(0xffffffffu, at < upto);
+      if (who == 0) {
+        at -= __shfl_sync(0xffffffffu, upto, 31);
+        continue;
+      }
+      const int src = __ffs(who) - 1, first = t0 + src * kEach;
+      at -= __shfl_sync(0xffffffffu, upto - mine, src);
+      c.token = first, each = __shfl_sync(0xffffffffu, units[0], src);
+#pragma unroll
+      for (int i = 1; i < kEach; ++i) {
+        const int further = __shfl_sync(0xffffffffu, units[i], src);
+        const int64_t of = static_cast<int64_t>(each) * a.kv_heads;
+        if (c.token == first + i - 1 && at >= of) at -= of, each = further, ++c.token;
+      }
+      break;
     }
-    const unsigned who = __ballot_sync(0xffffffffu, from < before + upto);
-    if (who != 0) {
-      const int src = __ffs(who) - 1, each = __shfl_sync(0xffffffffu, units, src);
-      const int64_t at = from - before - __shfl_sync(0xffffffffu, upto - mine, src);
-      c.token = t0 + src, c.tiles = each - kEntry;
-      c.kvh = static_cast<int>(divide(at, each));
-      const int in = static_cast<int>(at - static_cast<int64_t>(c.kvh) * each) - kEntry;
-      c.tile = in > 0 ? in : 0;
-      c.left = to - from + (in < 0 ? in : 0);
-      if (c.left < 0) c.left = 0;
-      return c;
-    }
-    before += __shfl_sync(0xffffffffu, upto, 31);
   }
+  if (each == 0) return c;
+  c.tiles = each - kEntry;
+  c.kvh = static_cast<int>(divide(at, each));
+  const int in = static_cast<int>(at - static_cast<int64_t>(c.kvh) * each) - kEntry;
+  c.tile = in > 0 ? in : 0;
+  c.left = to - from + (in < 0 ? in : 0);
+  if (c.left < 0) c.left = 0;
   return c;
 }
 // On to the warp's next tile; `context(token)`: what a change of tokens takes.  0: there is none (left is 0), 1: of the same item, 2: of another.
@@ -207,8 +273,9 @@ template <bool SPARSE, typename Context> __device__ __forceinline__ int advance(
 }
 
 // Scratch of a grid of `warps`: slot 2 b + 1 is for the item that warp b begins and does not end, slot 2 b for one begun before
-// it.  Accumulators [slots][group * dim], running maxima and sums [slots][8] of each; and for every item the warp that begins it and how
-// many warps have a part of it, which the one that begins it writes.
+// it.  Accumulators [slots][group * dim], running maxima and sums [slots][8] of each; and `shares`, which the warp that begins an item
+// writes.  By item: that warp and how many warps have a part of it.  By warp, where there are more items than warps: the item that it begins and
+// does not end (there is one at most), and how many have a part of it, 1 if there is none.
 struct Partials {
   float *acc, *m, *l;
   int2* shares;
@@ -239,10 +306,12 @@ kv8_attention_kernel(const __grid_constant__ Kv8Args a, const __grid_constant__ 
   const int grow = lane >> 2, quad = lane & 3;
   const int G = a.group;
   if (lane < a.tokens) prefetch_l1(a.sequence_ids + lane);  // needed once the token is known
-  const int64_t total = count_units<SPARSE>(a), warps = total < gridDim.x ? total : gridDim.x;
+  if (a.by_warp && lane == 0) Partials(a.scratch, gridDim.x, G * D).shares[blockIdx.x] = make_int2(0, 1);
+  const Line line = count_units<SPARSE>(a);
+  const int64_t total = line.total, warps = total < gridDim.x ? total : gridDim.x;
   if (blockIdx.x >= warps) return;
   const int64_t end_unit = divide(total * (blockIdx.x + 1), warps);
-  Cursor cur = find_unit<SPARSE>(a, divide(total * blockIdx.x, warps), end_unit);  // the tile that is computed next
+  Cursor cur = find_unit<SPARSE>(a, line, divide(total * blockIdx.x, warps), end_unit);  // the tile that is computed next
   if (cur.left == 0) return;
   Cursor next = cur;  // the tile that is fetched next, and what its rows are found by
   int64_t ctx = 0, coming_ctx = 0, coming_seq = 0;  // of the token, and of the one behind it
@@ -556,7 +625,9 @@ kv8_attention_kernel(const __grid_constant__ Kv8Args a, const __grid_constant__ 
   const size_t slot = 2 * static_cast<size_t>(blockIdx.x) + (first == 0 ? 1 : 0);
   if (first == 0 && lane == 0) {  // an item that others go on with ends cur.tiles - end units behind this warp's share
     const int last = whole ? blockIdx.x : static_cast<int>(((end_unit + cur.tiles - end) * warps - 1) / total);
-    part.shares[static_cast<int64_t>(token) * a.kv_heads + kvh] = make_int2(blockIdx.x, last - blockIdx.x + 1);
+    const int item = token * a.kv_heads + kvh, count = last - blockIdx.x + 1;
+    if (!a.by_warp) part.shares[item] = make_int2(blockIdx.x, count);
+    else if (!whole) part.shares[blockIdx.x] = make_int2(item, count);
   }
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
@@ -564,14 +635,13 @@ kv8_attention_kernel(const __grid_constant__ Kv8Args a, const __grid_constant__ 
     for (int sh = 4; sh < 32; sh <<= 1) l_run[e] += __shfl_xor_sync(0xffffffffu, l_run[e], sh);
     const int head = quad * 2 + e;
     if (head >= G) continue;
-    const float back = v_unit / (CENTRED ? 1.0f : Codec<C>::kUnit);
     if (whole) {
-#pragma unroll
-      for (int c = 0; c < NC; ++c)
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-          store_from_f32(out, token, (kvh * G + head) * D + c * 16 + 2 * grow + i, normalised(o[c][e + 2 * i] * back, l_run[e]), a.dtype);
+      // o / l, then the units, which keeps what is on the way in range
+      const float each = l_run[e] == 0.0f ? 0.0f : 1.0f / l_run[e];
+      store_dims<SPLIT>(out, token, static_cast<int64_t>(kvh * G + head) * D + 2 * grow, a.dtype, a.paired,
+                        [&](int c, int i) { return o[c][e + 2 * i] * each / (CENTRED ? 1.0f : Codec<C>::kUnit) * v_unit; }, std::integral_constant<int, NC>());
     } else {
+      const float back = v_unit / (CENTRED ? 1.0f : Codec<C>::kUnit);
       float* to = part.acc + (slot * G + head) * D + 2 * grow;
 #pragma unroll
       for (int c = 0; c < NC; ++c) *reinterpret_cast<float2*>(to + c * 16) = make_float2(o[c][e] * back, o[c][e + 2] * back);
@@ -586,7 +656,7 @@ kv8_attention_kernel(const __grid_constant__ Kv8Args a, const __grid_constant__ 
   }
 }
 
-// Adds the parts of one item: L lanes of four values each to a CTA, the threads / L groups of them every so many parts; the groups' sums meet
+// Adds the parts of an item, one for each entry of `shares`: L lanes of four values each to a CTA, the threads / L groups of them every so many parts; the groups' sums meet
 // in shared memory.  Always in the same order.  L: a warp where there are few items, so that many CTAs share an item; else what the
 // group * dim values take, at most all threads.
 template <int L>
@@ -602,6 +672,7 @@ kv8_attention_merge_kernel(const __grid_constant__ Kv8Args a, const __grid_const
   const Partials part(a.scratch, grid, all);
   const int2 share = __ldcg(part.shares + blockIdx.x);
   if (share.y == 1) return;  // the same for all threads
+  const int item = a.by_warp ? share.x : blockIdx.x, begins = a.by_warp ? blockIdx.x : share.x;
   const bool some = at < all;
   const int head = some ? at / dim : 0;
   float m = -INFINITY, l = 0.0f;
@@ -614,7 +685,7 @@ kv8_attention_merge_kernel(const __grid_constant__ Kv8Args a, const __grid_const
   };
 #pragma unroll 8
   for (int i = group; i < share.y; i += kGroups) {
-    const size_t slot = 2 * static_cast<size_t>(share.x + i) + (i == 0 ? 1 : 0);
+    const size_t slot = 2 * static_cast<size_t>(begins + i) + (i == 0 ? 1 : 0);
     const float4 v = some ? __ldcg(reinterpret_cast<const float4*>(part.acc + slot * all + at)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     add(v, __ldcg(part.m + slot * kMaxGroup + head), __ldcg(part.l + slot * kMaxGroup + head));
   }
@@ -625,7 +696,7 @@ kv8_attention_merge_kernel(const __grid_constant__ Kv8Args a, const __grid_const
     for (int w = 1; w < kGroups; ++w) add(accs[w][lane], ms[w][lane], ls[w][lane]);
   }
   if (!some) return;
-  const int token = blockIdx.x / a.kv_heads, kvh = blockIdx.x - token * a.kv_heads;
+  const int token = item / a.kv_heads, kvh = item - token * a.kv_heads;
   const int64_t col = static_cast<int64_t>(kvh) * all + at;
   store_from_f32(out, token, col, normalised(acc.x, l), a.dtype);
   store_from_f32(out, token, col + 1, normalised(acc.y, l), a.dtype);
@@ -648,12 +719,13 @@ int grid_for(int64_t items, int64_t dim, int64_t tiles) {
 int64_t hint_tiles(int64_t context, int64_t dim) { return ((context < 1 ? kMaxContextHint : context) + tile_of(dim) - 1) / tile_of(dim); }
 
 template <typename C, int D, bool SPLIT, bool SPARSE>
-int launch_kv8(const Kv8Args& a, const PeerOut& out, int warps, cudaStream_t s) {
+int launch_kv8(Kv8Args a, const PeerOut& out, int warps, cudaStream_t s) {
+  const int items = a.tokens * a.kv_heads, lanes = a.group * D / 4;
+  a.by_warp = items > warps;
   if (int st = launch_dependent(kv8_attention_kernel<C, D, SPLIT, SPARSE>, dim3(static_cast<unsigned>(warps)), dim3(32), ring_bytes<D>(), s, a, out))
     return st;
-  const int items = a.tokens * a.kv_heads, lanes = a.group * D / 4;
   auto merge = [&](auto kernel, int l) {
-    return launch_opts(kernel, dim3(static_cast<unsigned>(items), static_cast<unsigned>((lanes + l - 1) / l)), dim3(kMergeThreads), 0, s, 1u, true, a, out,
+    return launch_opts(kernel, dim3(static_cast<unsigned>(a.by_warp ? warps : items), static_cast<unsigned>((lanes + l - 1) / l)), dim3(kMergeThreads), 0, s, 1u, true, a, out,
                        D, warps);
   };
   if (items <= sm_count() || lanes <= 32) return merge(kv8_attention_merge_kernel<32>, 32);
@@ -696,6 +768,8 @@ int kv8_arguments(const void* q, const void* k_cache, const void* v_cache, const
   a->hnd = hnd ? 1 : 0;
   a->narrow = page_size * max_pages < (1LL << 31) ? 1 : 0;
   a->scale = scale;
+  a->paired = out->ld % 2 == 0 && out->col0 % 2 == 0;
+  for (int p = 0; p < out->world; ++p) a->paired &= reinterpret_cast<uintptr_t>(out->ptr[p]) % (dtype == XDK_F32 ? 8 : 4) == 0;
   a->tile = tile_of(head_dim);
   return XDK_OK;
 }

@@ -529,13 +529,15 @@ def test_streams_and_a_wider_destination():
         chosen = kv8.select_kv8_pages(late, ours, *args, top_pages=9)
     stream.synchronize()
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]) and torch.equal(chosen, pages)
-    wide = torch.full((2, 600), -7.0, dtype=F16, device="cuda")
-    dst = _native.PeerOutStruct()
-    dst.ptr[0], dst.world, dst.ld, dst.col0 = wide.data_ptr(), 1, 600, 40
-    assert kv8.paged_kv8_decode_attention(q, ours, *args, peer_out=dst) is None
-    assert torch.equal(wide[:, 40:552], want[0].view(2, 512)) and (wide[:, :40] == -7).all() and (wide[:, 552:] == -7).all()
-    kv8.paged_kv8_sparse_attention(q, ours, pages, *args, peer_out=dst)
-    assert torch.equal(wide[:, 40:552], want[1].view(2, 512))
+    for width, col in ((600, 40), (601, 40), (600, 41)):  # rows that begin on any element
+        wide = torch.full((2, width), -7.0, dtype=F16, device="cuda")
+        dst = _native.PeerOutStruct()
+        dst.ptr[0], dst.world, dst.ld, dst.col0 = wide.data_ptr(), 1, width, col
+        assert kv8.paged_kv8_decode_attention(q, ours, *args, peer_out=dst) is None
+        mine = slice(col, col + 512)
+        assert torch.equal(wide[:, mine], want[0].view(2, 512)) and (wide[:, :col] == -7).all() and (wide[:, col + 512:] == -7).all()
+        kv8.paged_kv8_sparse_attention(q, ours, pages, *args, peer_out=dst)
+        assert torch.equal(wide[:, mine], want[1].view(2, 512)) and (wide[:, :col] == -7).all() and (wide[:, col + 512:] == -7).all()
 
 
 def test_two_streams_at_once():
