@@ -403,23 +403,23 @@ kv8_append_kernel(const __grid_constant__ AppendArgs a, int block_rows) {
   for (int d = lane * 4; d < D; d += 32 * 4) write_mean<C, D>(a, b, d);
 }
 
-// Longer batches, first launch: the first `entries` CTAs enter every token's page into the table, the next `q_blocks` rotate Q, the others
-// find the largest values of K and V.
+// The token and the unit in it of thread t of CTA `cta`, `per_token` units to a token.
+__device__ __forceinline__ int2 token_and_unit(int64_t cta, int per_token) {
+  const int64_t first = cta * kThreads;
+  int token = static_cast<int>(first / per_token), unit = static_cast<int>(first - static_cast<int64_t>(token) * per_token) + threadIdx.x;
+  const int further = unit / per_token;
+  return make_int2(token + further, unit - further * per_token);
+}
+// Longer batches, first launch: the first `entries` CTAs enter every token's page into the table, the others find the largest values of K
+// and V.
 template <typename T, int D, bool VEC>
 __global__ void __launch_bounds__(kThreads)
-kv8_group_kernel(const __grid_constant__ AppendArgs a, const __grid_constant__ Groups g, unsigned entries, unsigned q_blocks) {
+kv8_group_kernel(const __grid_constant__ AppendArgs a, const __grid_constant__ Groups g, unsigned entries) {
   pdl_launch_dependents();
   pdl_wait();
   if (blockIdx.x >= entries) {
-    const bool is_q = blockIdx.x < entries + q_blocks;
-    const int64_t first = static_cast<int64_t>(blockIdx.x - (is_q ? entries : entries + q_blocks)) * kThreads;  // unit of thread 0
-    const int per_token = is_q ? units_of<T, D>(a.q_heads) : 2 * units_of<T, D>(a.kv_heads);
-    int token = static_cast<int>(first / per_token);
-    int unit = static_cast<int>(first - static_cast<int64_t>(token) * per_token) + threadIdx.x;
-    const int further = unit / per_token;
-    token += further, unit -= further * per_token;
-    if (!is_q) find_tops<T, D, VEC>(a, g.tops, token < a.tokens ? token : 0, unit, token < a.tokens);
-    else if (token < a.tokens) rotate_q<T, D, VEC>(a, token, unit);
+    const int2 at = token_and_unit(blockIdx.x - entries, 2 * units_of<T, D>(a.kv_heads));
+    find_tops<T, D, VEC>(a, g.tops, at.x < a.tokens ? at.x : 0, at.y, at.x < a.tokens);
     return;
   }
   const int token = blockIdx.x * kThreads + threadIdx.x;
@@ -448,22 +448,31 @@ kv8_group_kernel(const __grid_constant__ AppendArgs a, const __grid_constant__ G
   g.slot_of[token] = slot;
 }
 
-// Second launch: CTAs take four blocks of a page in the table in turn.  A warp finds the scale of one, then all threads write the rows of
-// all four.
+// Second launch: `block_ctas` CTAs take four blocks of a page in the table in turn.  A warp finds the scale of one, then all threads write
+// the rows of all four.  Between them `q_ctas` CTAs rotate Q, which keeps HBM busy while those wait for their chains of loads.
 template <typename T, typename C, int D, bool VEC>
 __global__ void __launch_bounds__(kThreads)
-kv8_blocks_kernel(const __grid_constant__ AppendArgs a, const __grid_constant__ Groups g, unsigned parts) {
+kv8_blocks_kernel(const __grid_constant__ AppendArgs a, const __grid_constant__ Groups g, unsigned parts, unsigned block_ctas, unsigned q_ctas) {
   constexpr int kWarps = kThreads / 32, kPerRow = D / 16;
   extern __shared__ int token_of[];  // [page_size]
   __shared__ Block blocks[kWarps];
   pdl_launch_dependents();
+  // in turn, then what is left of either kind
+  const unsigned both = 2 * (block_ctas < q_ctas ? block_ctas : q_ctas);
+  const bool is_q = blockIdx.x < both ? (blockIdx.x & 1) != 0 : block_ctas < q_ctas;
+  const unsigned cta = blockIdx.x < both ? blockIdx.x / 2 : blockIdx.x - both / 2;
+  if (is_q) {  // no wait: nothing of the first launch is read, which began when all work before it had ended
+    const int2 at = token_and_unit(cta, units_of<T, D>(a.q_heads));
+    if (at.x < a.tokens) rotate_q<T, D, VEC>(a, at.x, at.y);
+    return;
+  }
   pdl_wait();
-  const unsigned part = blockIdx.x % parts;  // of a page's blocks; the grid: a multiple of them
+  const unsigned part = cta % parts;  // of a page's blocks; block_ctas is a multiple of them
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, heads = 2 * a.kv_heads;
   const int head = part * kWarps + warp, some = heads - static_cast<int>(part) * kWarps < kWarps ? heads - part * kWarps : kWarps;
   int d0, d1;
   dims_of<VEC>(a, threadIdx.x % kPerRow, d0, d1);
-  for (unsigned entry = blockIdx.x / parts; entry <= g.mask; entry += gridDim.x / parts) {
+  for (unsigned entry = cta / parts; entry <= g.mask; entry += block_ctas / parts) {
     const int slot = g.list[entry];
     if (slot < 0) return;  // behind the last one; the same for all threads
     for (int i = threadIdx.x; i < a.page_size; i += kThreads) token_of[i] = -1;
@@ -515,17 +524,17 @@ int launch_append(const AppendArgs& a, void* scratch, cudaStream_t stream) {
                             stream, a, static_cast<int>(parts));
   }
   const Groups g = groups_at(scratch, a.tokens, a.kv_heads);
-  if (int st = note_launch(cudaMemsetAsync(scratch, 0xff, cleared_bytes(a.tokens), stream))) return st;
-  const int64_t entries = (a.tokens + kThreads - 1) / kThreads, q_blocks = (a.tokens * q_units + kThreads - 1) / kThreads;
-  const int64_t kv_blocks = (a.tokens * 2 * units_of<T, D>(a.kv_heads) + kThreads - 1) / kThreads;
-  if (entries + q_blocks + kv_blocks > 2147483647LL) return XDK_ERR_LIMIT;
-  if (int st = launch_opts(kv8_group_kernel<T, D, VEC>, dim3(static_cast<unsigned>(entries + q_blocks + kv_blocks)), dim3(kThreads), 0, stream, 1u,
-                           false, a, g, static_cast<unsigned>(entries), static_cast<unsigned>(q_blocks)))
-    return st;
+  const int64_t entries = (a.tokens + kThreads - 1) / kThreads, q_ctas = (a.tokens * q_units + kThreads - 1) / kThreads;
+  const int64_t kv_ctas = (a.tokens * 2 * units_of<T, D>(a.kv_heads) + kThreads - 1) / kThreads;
   // as many CTAs as there can be work for, or the SMs hold
-  const int64_t wave = (static_cast<int64_t>(sm_count()) * 8 + parts - 1) / parts;
-  return launch_opts(kv8_blocks_kernel<T, C, D, VEC>, dim3(static_cast<unsigned>((a.tokens < wave ? a.tokens : wave) * parts)), dim3(kThreads), map,
-                     stream, 1u, true, a, g, static_cast<unsigned>(parts));
+  const int64_t wave = (static_cast<int64_t>(sm_count()) * 8 + parts - 1) / parts, block_ctas = (a.tokens < wave ? a.tokens : wave) * parts;
+  if (entries + kv_ctas > 2147483647LL || block_ctas + q_ctas > 2147483647LL) return XDK_ERR_LIMIT;
+  if (int st = note_launch(cudaMemsetAsync(scratch, 0xff, cleared_bytes(a.tokens), stream))) return st;
+  if (int st = launch_opts(kv8_group_kernel<T, D, VEC>, dim3(static_cast<unsigned>(entries + kv_ctas)), dim3(kThreads), 0, stream, 1u, false, a, g,
+                           static_cast<unsigned>(entries)))
+    return st;
+  return launch_opts(kv8_blocks_kernel<T, C, D, VEC>, dim3(static_cast<unsigned>(block_ctas + q_ctas)), dim3(kThreads), map, stream, 1u, true, a, g,
+                     static_cast<unsigned>(parts), static_cast<unsigned>(block_ctas), static_cast<unsigned>(q_ctas));
 }
 
 template <typename T, typename C>
