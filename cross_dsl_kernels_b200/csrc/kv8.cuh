@@ -14,13 +14,12 @@ struct E4m3Codes {};
 template <typename C> struct Codec;
 template <> struct Codec<Int8Codes> {
   static constexpr float kTop = 127.0f;
-  // round half to even, at most kTop (a quotient passes it where the scale is subnormal)
+  // Round half to even: the sum with 1.5 * 2^23 is a whole number, whose low byte is the code's.  |x| <= kTop.
   __device__ static __forceinline__ uint32_t pack4(const float* x) {
-    uint32_t v = 0;
+    uint32_t v[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      v |= (static_cast<uint32_t>(static_cast<int>(fminf(fmaxf(rintf(x[i]), -kTop), kTop))) & 0xffu) << (8 * i);
-    return v;
+    for (int i = 0; i < 4; ++i) v[i] = __float_as_uint(__fadd_rn(x[i], 12582912.0f));
+    return __byte_perm(__byte_perm(v[0], v[1], 0x0040), __byte_perm(v[2], v[3], 0x0040), 0x5410);
   }
   __device__ static __forceinline__ void unpack4(uint32_t v, float* x) {
 #pragma unroll

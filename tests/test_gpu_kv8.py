@@ -118,6 +118,21 @@ def test_append_chunks_in_any_order(codes, tokens, order):
                 interleaved=False)
 
 
+@pytest.mark.parametrize("codes", [INT8, E4M3])
+@pytest.mark.parametrize("heads,dim,page", [((4, 2), 64, 40), ((2, 1), 256, 24), ((9, 3), 128, 64), ((6, 6), 64, 7), ((3, 3), 256, 33)])
+def test_append_long_chunks_of_any_page(codes, heads, dim, page):
+    """Prompts that fill some pages and end inside others, then their next chunk: pages of few and of many rows."""
+    g, lens, layout = _gen(dim + page), [210, 90], "HND" if page % 2 else "NHD"
+    per_seq = -(-2 * max(lens) // page)
+    table, cache = _table(2, per_seq, 3), oracle.empty(2 * per_seq, page, heads[1], dim, codes)
+    ours, trig = _on_gpu(cache, layout), _trig(2 * max(lens), dim)
+    seq = torch.cat([torch.full((n,), i) for i, n in enumerate(lens)])
+    for chunk in range(2):
+        pos = torch.cat([torch.arange(n) + chunk * n for n in lens])
+        _append(ours, cache, *(_values(300, h, dim, F16, g, 1.0) for h in (heads[0], heads[1], heads[1])), trig, pos, table, seq, rope_dim=dim,
+                interleaved=False)
+
+
 @pytest.mark.parametrize("tokens", [9, 200])
 def test_append_several_tokens_for_one_slot(tokens):
     """Of tokens for the same slot the last one counts, in every launch form."""
