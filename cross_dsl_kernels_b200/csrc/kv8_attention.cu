@@ -21,8 +21,11 @@
 // HBM-bound in the long run.  The tiles of 32 positions of all (token, KV head) items stand in one line, and every warp -- a CTA of its own, as
 // many as the SMs hold -- takes an equal range: no barrier but the warp's, and its ring of cp.async stages never runs dry, not at
 // the end of an item either.  Items that several warps share leave one partial result per warp in scratch, which a second launch adds in
-// their order.  (Chunks that the hardware hands out as warps finish, by CTAs or by cancelled launches, measured slower: 70 us against 61
-// for 16 contexts of 8192; a chunk's start costs its warp 6 us without loads.)
+// their order.  (Chunks that the hardware hands out as warps finish, by CTAs or by cancelled launches, measured slower: 70 us for 16
+// contexts of 8192, where equal ranges took 61 with the same tiles; a chunk's start costs its warp 6 us without loads.)
+//
+// 32 / 8 heads of 128, us: 16 contexts of 32768 172 (6.2 TB/s), of 8192 57 (4.7), 64 of 1 .. 2048 37, one of 8192 14.5.  Of short work it is bound by
+// its two launches and the chain position -> page table -> rows (8 us), of long work by HBM.
 #include <math.h>
 
 #include <type_traits>
@@ -166,8 +169,8 @@ __device__ __forceinline__ float normalised(float acc, float l) { return l == 0.
 // ---- the line of tiles ---------------------------------------------------------------------------------------------------
 // Token by token, its KV heads; to each kEntry units and one for every tile of the context (one dead tile for an empty one).  Only the
 // device knows the contexts: each warp adds them up.  Warp b of B has the tiles among units [b U / B, (b + 1) U / B) of the U there are, B:
-// the warps of the grid, or U if that is less.  (Without the entries a warp among contexts of a tile or two had nine of them to begin and
-// to end: 72 us for 64 contexts of 1 .. 2048, where 64 of 1024 took 38.)
+// the warps of the grid, or U if that is less.  (Without the entries a warp among contexts of a tile or two has nine of them to begin and
+// to end: 64 contexts of 1 .. 2048 took 72 us then, 44 with them.)
 struct Cursor {
   int token, kvh, tile, tiles;
   int64_t left;  // units of the warp from this tile on

@@ -40,7 +40,7 @@ class PagedKV8Cache:
     """Codes, scales and mean keys of a paged cache; the tensors are the caller's and are written in place.
 
     ``k``, ``v``: int8 or float8_e4m3fn, [pages, page_size, kv_heads, head_dim] ("NHD") or [pages, kv_heads, page_size, head_dim]
-    ("HND"); ``k_scale``, ``v_scale``: float32 [pages, kv_heads], a value is code * scale; ``k_mean``: int8 [pages, kv_heads,
+    ("HND"); ``k_scale``, ``v_scale``: float32 [pages, kv_heads], a value is code * scale, and no scale is negative; ``k_mean``: int8 [pages, kv_heads,
     head_dim], the mean key of each full block in units of its scale (e4m3: of its scale * 448 / 127), or None for a cache from
     which no pages are selected."""
 

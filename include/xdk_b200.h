@@ -306,8 +306,8 @@ XDK_API int xdk_swiglu_peer(const void* upgate, const xdk_peer_out* out_dst, int
 /*
  * The paged K/V cache in 8 bits (no counterpart in the reference): half the bytes of a 16-bit one.  Codes of one byte, int8 or
  * e4m3, in the two cache layouts of xdk_rope_kv_append, and per block -- a page of one KV head -- an FP32 scale for K and one for V,
- * [pages, kv_heads]: a value is code * scale.  k_mean, int8 [pages, kv_heads, head_dim], holds the mean key of each block, for
- * the selection of pages.  head_dim in {64, 128, 256}, page_size <= 1024; caches, k_mean, scratch 16-byte aligned.
+ * [pages, kv_heads]: a value is code * scale, and no scale is negative.  k_mean, int8 [pages, kv_heads, head_dim], holds the mean key
+ * of each block, for the selection of pages.  head_dim in {64, 128, 256}, page_size <= 1024; caches, k_mean, scratch 16-byte aligned.
  *
  * xdk_kv8_append: the rotation and the append of xdk_rope_kv_append, in any order of tokens and any number of them for a page.  For each
  *   block, with W its rows that the call writes, top = 127 (int8) or 448 (e4m3):

@@ -9,6 +9,8 @@ references (paths are relative to the upstream project):
 * src/crossdsl_kernels/references/paged_address.py -> :mod:`oracle.paging`
 * src/crossdsl_kernels/quantization.py         -> :mod:`oracle.int4`
 
+:mod:`oracle.kv8` states the 8-bit paged cache, which upstream does not have.
+
 Only the test-suite, the smoke check and the benchmark's CPU-baseline leg may
 import it.  The shipped library (``cross_dsl_kernels_b200``) never does: its
 ops run on the GPU or raise.
