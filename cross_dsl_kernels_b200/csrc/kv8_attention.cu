@@ -719,7 +719,9 @@ int grid_for(int64_t items, int64_t dim, int64_t tiles) {
   const int64_t all = items * ((tiles < 1 ? 1 : tiles) + kEntry), warps = all < most ? all : most, each = (all + warps - 1) / warps;
   return static_cast<int>((all + each - 1) / each);
 }
-int64_t hint_tiles(int64_t context, int64_t dim) { return ((context < 1 ? kMaxContextHint : context) + tile_of(dim) - 1) / tile_of(dim); }
+int64_t hint_tiles(int64_t context, int64_t dim) {
+  return ((context < 1 || context > kMaxContextHint ? kMaxContextHint : context) + tile_of(dim) - 1) / tile_of(dim);
+}
 
 template <typename C, int D, bool SPLIT, bool SPARSE>
 int launch_kv8(Kv8Args a, const PeerOut& out, int warps, cudaStream_t s) {

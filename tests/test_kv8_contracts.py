@@ -111,7 +111,7 @@ def test_c_entry_points_check_sizes_before_they_touch_a_gpu():
         assert append(**kw) in (limit, wrong), kw
     assert lib.xdk_kv8_append_scratch_bytes(128, 2) == 0 and lib.xdk_kv8_append_scratch_bytes(129, 2) >= 512 * 20
     size = lib.xdk_kv8_decode_attention_scratch_bytes
-    assert 0 < size(1, 4, 2, 64, 1024) < size(1, 4, 2, 64, 8192) <= size(1, 4, 2, 64, 0) == size(1, 4, 2, 64, 1 << 62)
+    assert 0 < size(1, 4, 2, 64, 1024) < size(1, 4, 2, 64, 8192) <= size(1, 4, 2, 64, 0) == size(1, 4, 2, 64, 1 << 62) == size(1, 4, 2, 64, (1 << 63) - 1)
     assert size(1, 18, 2, 64, 8192) == size(0, 4, 2, 64, 64) == size(1, 4, 2, 96, 64) == size(1, 4, 3, 64, 64) == 0
     assert lib.xdk_kv8_sparse_attention_scratch_bytes(1, 4, 2, 64, 16, 8) > 0 == lib.xdk_kv8_sparse_attention_scratch_bytes(1, 4, 2, 64, 16, 0)
 
