@@ -7,13 +7,13 @@
 // the same whatever computes it.  One choice per token and KV head: the query heads that share it read its pages together.
 //
 // One CTA per (token, KV head).  Scores: mma.m16n8k32 on bytes, 16 pages as rows, the heads of the group as columns; a thread
-// loads a quarter of two pages' means with 16-byte loads, four threads 64 bytes in a row (14.0 us for 16 tokens, 8 KV heads and
-// 2048 pages; a quarter of the dims in a row to each thread: 14.5), those of four blocks of 16 pages at a time (the next four loaded
-// during these ones' products: 14.7), and the codes of q stand in registers in the same order of dims.  The scores stay in shared
+// loads a quarter of two pages' means with 16-byte loads, four threads 64 bytes in a row (14.0 us for 16 tokens, 8 KV heads and 2048
+// pages that L2 holds in part; a quarter of the dims in a row to each thread: 14.5), those of four blocks of 16 pages at a time (the next four
+// loaded during these ones' products: 14.7), and the codes of q stand in registers in the same order of dims.  The scores stay in shared
 // memory as sortable integers; up to three passes over 11, 11 and 10 bits of them find the value of the last one chosen (two, mostly:
 // no other has its first 22 bits), one more writes the pages in order.
-// Bound: 512 pages (7.3 us for one token) by the chain of loads and barriers; 2048 pages, whose means are 35 MB, by the latency of
-// their reads: 2.3 us in front of the scores, 8.4 for them, 3.3 for the choice.
+// Bound: 512 pages (7.0 us for one token) by the chain of loads and barriers; 2048 pages, whose means are 35 MB, from HBM (15.6 us) by
+// the latency of their reads: 2.3 us in front of the scores, 10 for them, 3.3 for the choice.
 #include <math.h>
 
 #include "kv8.cuh"
