@@ -24,7 +24,7 @@
 // their order.  (Chunks that the hardware hands out as warps finish, by CTAs or by cancelled launches, measured slower: 70 us for 16
 // contexts of 8192, where equal ranges took 61 with the same tiles; a chunk's start costs its warp 6 us without loads.)
 //
-// 32 / 8 heads of 128, us: 16 contexts of 32768 172 (6.2 TB/s), of 8192 57 (4.7), 64 of 1 .. 2048 37, one of 8192 16.  Of short work it is bound by
+// 32 / 8 heads of 128, us: 16 contexts of 32768 172 (6.2 TB/s), of 8192 57 (4.7), 64 of 1 .. 2048 37, one of 8192 14.  Of short work it is bound by
 // its two launches and the chain position -> page table -> rows (8 us), of long work by HBM.
 #include <math.h>
 
@@ -57,7 +57,6 @@ constexpr int kMaxGroup = 8;                 // heads of a group: columns of a m
 template <int D> constexpr int kTileOf = D == 64 ? 64 : 32;  // positions of a tile: of 8 KB or more
 inline int tile_of(int64_t dim) { return dim == 64 ? kTileOf<64> : kTileOf<128>; }
 constexpr int kEntry = 2;                    // what the change to another item costs a warp, in tiles
-constexpr int kMergeThreads = 256;
 constexpr int64_t kMaxContextHint = 1LL << 38;
 constexpr float kWeightLog2 = 14.0f;            // the largest weight of a head in FP16 is 2^14
 constexpr float kLeastScale = 8.0779357e-28f;   // 2^-90: scales of V below that, in units of the first tile's, count as that
@@ -659,13 +658,13 @@ kv8_attention_kernel(const __grid_constant__ Kv8Args a, const __grid_constant__ 
   }
 }
 
-// Adds the parts of an item, one for each entry of `shares`: L lanes of four values each to a CTA, the threads / L groups of them every so many parts; the groups' sums meet
-// in shared memory.  Always in the same order.  L: a warp where there are few items, so that many CTAs share an item; else what the
-// group * dim values take, at most all threads.
-template <int L>
-__global__ void __launch_bounds__(kMergeThreads)
+// Adds the parts of an item, one for each entry of `shares`: L lanes of four values each to a CTA, the THREADS / L groups of them every so
+// many parts; the groups' sums meet in shared memory.  Always in the same order.  L: a warp where there are few items, so that many CTAs
+// share an item; else what the group * dim values take, at most all threads.
+template <int L, int THREADS>
+__global__ void __launch_bounds__(THREADS)
 kv8_attention_merge_kernel(const __grid_constant__ Kv8Args a, const __grid_constant__ PeerOut out, int dim, int grid) {
-  constexpr int kGroups = kMergeThreads / L;
+  constexpr int kGroups = THREADS / L;
   __shared__ float4 accs[kGroups][L];
   __shared__ float ms[kGroups][L], ls[kGroups][L];
   pdl_launch_dependents();
@@ -729,12 +728,16 @@ int launch_kv8(Kv8Args a, const PeerOut& out, int warps, cudaStream_t s) {
   a.by_warp = items > warps;
   if (int st = launch_dependent(kv8_attention_kernel<C, D, SPLIT, SPARSE>, dim3(static_cast<unsigned>(warps)), dim3(32), ring_bytes<D>(), s, a, out))
     return st;
-  auto merge = [&](auto kernel, int l) {
-    return launch_opts(kernel, dim3(static_cast<unsigned>(a.by_warp ? warps : items), static_cast<unsigned>((lanes + l - 1) / l)), dim3(kMergeThreads), 0, s, 1u, true, a, out,
-                       D, warps);
+  const int entries = a.by_warp ? warps : items;
+  auto merge = [&](auto kernel, int l, int threads) {
+    return launch_opts(kernel, dim3(static_cast<unsigned>(entries), static_cast<unsigned>((lanes + l - 1) / l)), dim3(threads), 0, s, 1u, true, a, out, D,
+                       warps);
   };
-  if (items <= sm_count() || lanes <= 32) return merge(kv8_attention_merge_kernel<32>, 32);
-  return lanes <= 128 ? merge(kv8_attention_merge_kernel<128>, 128) : merge(kv8_attention_merge_kernel<256>, 256);
+  // at most one CTA to an SM: of 512 threads, sixteen parts at once (one context of 8192, 130 parts a head: 15.9 -> 13.9 us; in more CTAs than
+  // that 256 threads are faster, 57.5 against 58.9 for 16 of them)
+  if (entries * ((lanes + 31) / 32) <= sm_count()) return merge(kv8_attention_merge_kernel<32, 512>, 32, 512);
+  if (entries <= sm_count() || lanes <= 32) return merge(kv8_attention_merge_kernel<32, 256>, 32, 256);
+  return lanes <= 128 ? merge(kv8_attention_merge_kernel<128, 256>, 128, 256) : merge(kv8_attention_merge_kernel<256, 256>, 256, 256);
 }
 
 template <typename C, bool SPARSE>
