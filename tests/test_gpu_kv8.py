@@ -527,6 +527,28 @@ def test_all_pages_selected_is_the_whole_context():
     _close(kv8.paged_kv8_sparse_attention(q.cuda(), ours, pages, *args), exact, F16, 128)
 
 
+@pytest.mark.parametrize("tokens", [7, 200])
+def test_padding_names_no_sequence(tokens):
+    """A padded batch: what stands in the sequence ids of padding, and in the page table behind a context, is nothing that is read."""
+    from cross_dsl_kernels_b200 import kv8
+    heads, dim, page, g = (4, 2), 128, 16, _gen(21)
+    cache, table = _filled(30, page, 2, dim, INT8, 21), torch.full((2, 40), 1 << 40)
+    table[:, :15] = torch.randperm(30, generator=g).reshape(2, 15)
+    pos, seq = torch.full((tokens,), -1), torch.full((tokens,), 1 << 50)
+    pos[2:7:2], seq[2:7:2] = torch.tensor([100, 239, 16]), torch.tensor([0, 1, 1])
+    pos[0] = -(1 << 40)
+    seq[3] = -9
+    ours = _on_gpu(cache, "NHD")
+    q, k, v = (torch.randn(tokens, h, dim, generator=g).half() for h in (4, 2, 2))
+    q = _append(ours, cache, q, k, v, _trig(256, dim), pos, table, seq, rope_dim=dim, interleaved=False)
+    args = [t.cuda() for t in (pos, table, seq)]
+    pages = kv8.select_kv8_pages(q, ours, *args, top_pages=3)
+    assert torch.equal(pages.cpu(), oracle.select(q.cpu(), cache, pos, table, seq, top_pages=3))
+    for got, kept in ((kv8.paged_kv8_decode_attention(q, ours, *args), None), (kv8.paged_kv8_sparse_attention(q, ours, pages, *args), pages.cpu())):
+        _close(got, oracle.attention(q.cpu(), cache, pos, table, seq, pages=kept), F16, dim)
+        assert (got[(pos < 0).cuda()] == 0).all()
+
+
 def test_streams_and_a_wider_destination():
     """On a stream that is not the default one, behind work that is still running there; and the output as columns of a wider matrix."""
     from cross_dsl_kernels_b200 import _native, kv8
