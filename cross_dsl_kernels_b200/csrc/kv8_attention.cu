@@ -428,6 +428,10 @@ kv8_attention_kernel(const __grid_constant__ Kv8Args a, const __grid_constant__ 
   }
   uint32_t qb[NQ][NC][2];  // q^T as B fragments: dims 16 c + 4 quad + {0,1}, {2,3} of head grow
   float unit[2];           // of the scores of heads 2 quad + {0, 1}: scale * log2(e) * the power of two that q was divided by
+  // Codes that are not centred are multiples of kUnit, by which the units of the scores are divided, or, beside a q above 2^37, the scales of
+  // K are multiplied: the quotient of either would not always be finite, and beside such a q a scale of K above 2^104 gives no finite score.
+  constexpr float kPerUnit = CENTRED ? 1.0f : 1.0f / Codec<C>::kUnit;
+  float k_lift = 1.0f;
   {
     float top = 0.0f;
 #pragma unroll
@@ -455,9 +459,13 @@ kv8_attention_kernel(const __grid_constant__ Kv8Args a, const __grid_constant__ 
           qb[NQ - 1][c][h] = Mma16816<__half>::pack(x0 - f.x, x1 - f.y);
         }
       }
+    float per_unit = a.scale * 1.4426950408889634f;
+    if constexpr (kPerUnit != 1.0f) {
+      if (__any_sync(0xffffffffu, exponent > 36)) k_lift = kPerUnit;
+      else per_unit *= kPerUnit;
+    }
 #pragma unroll
-    for (int e = 0; e < 2; ++e)
-      unit[e] = __shfl_sync(0xffffffffu, back, (2 * quad + e) * 4) * (a.scale * 1.4426950408889634f / (CENTRED ? 1.0f : Codec<C>::kUnit));
+    for (int e = 0; e < 2; ++e) unit[e] = __shfl_sync(0xffffffffu, back, (2 * quad + e) * 4) * per_unit;
   }
   float s_zero[2] = {0.0f, 0.0f};  // what a score begins with: codes that are not centred add kOffset * q
   if constexpr (!CENTRED && Codec<C>::kOffset != 0.0f) {
@@ -507,7 +515,7 @@ kv8_attention_kernel(const __grid_constant__ Kv8Args a, const __grid_constant__ 
       float rel = __fdividef(vs[0][r], v_unit);
       rel = rel < kLeastScale ? kLeastScale : rel;  // NaN passes
       const float in_exponent = log2_fast(rel);
-      per_row[r * 32 + lane] = make_float4(ks[0][r], live ? in_exponent : -INFINITY, live ? exp2_fast(-in_exponent) : 0.0f, 0.0f);
+      per_row[r * 32 + lane] = make_float4(ks[0][r] * k_lift, live ? in_exponent : -INFINITY, live ? exp2_fast(-in_exponent) : 0.0f, 0.0f);
 #pragma unroll
       for (int s = 0; s < NST - 1; ++s) ks[s][r] = ks[s + 1][r], vs[s][r] = vs[s + 1][r];
     }
