@@ -8,9 +8,10 @@
 // heads of the group as the 8 columns:
 //   * q is scaled by a power of two, so that its largest value is near 2^14, and rounded to FP16 (FP16 and BF16 values pass whole unless
 //     they are 2^-27 of the largest); an FP32 q is the sum of two such numbers, and each product two products.
-//   * the weights are the softmax weights times the block scales of V, w = p * vs = 2^(s + log2 vs): one running maximum, of the whole
-//     exponent, keeps them in range whatever the scales are (down to 2^-90 of the first tile's); the softmax sum takes vs out again.  The largest
-//     weight of a head is 2^14, so that what rounds away is below 2^-38 of it; weights are rounded to FP16 (half a step: 2^-11), for FP32
+//   * the weights are the softmax weights times the block scales of V, w = p * vs = 2^(s + e) * f with vs = 2^e * f, f in [1, 2): the running
+//     maximum of s + e keeps them in range whatever the scales are, that of s alone the sum of the softmax weights.  (One maximum and one exponential
+//     for both, the sum with vs taken out again, holds for scales within 2^60 of one another; it takes the same time.)  The largest
+//     weight of a head is 2^14 or more, so that what rounds away is below 2^-38 of it; weights are rounded to FP16 (half a step: 2^-11), for FP32
 //     again as the sum of two.
 //   * int8 codes enter as the subnormal halves (code + 128) * 2^-24, which a byte permute makes; the sums begin with -128 times the sum of
 //     the other operand.  FP32 results would see the few 2^-23 of 128 that this rounds away: for them the codes are centred first.
@@ -20,8 +21,8 @@
 //
 // HBM-bound in the long run.  The tiles of 32 positions of all (token, KV head) items stand in one line, and every warp -- a CTA of its own, as
 // many as the SMs hold -- takes an equal range: no barrier but the warp's, and its ring of cp.async stages never runs dry, not at
-// the end of an item either.  Items that several warps share leave one partial result per warp in scratch, which a second launch adds in
-// their order.  (Chunks that the hardware hands out as warps finish, by CTAs or by cancelled launches, measured slower: 70 us for 16
+// the end of an item either.  Of an item that several warps share each leaves the result over its positions in scratch, with its share of the
+// weights, and a second launch adds them in their order.  (Chunks that the hardware hands out as warps finish, by CTAs or by cancelled launches, measured slower: 70 us for 16
 // contexts of 8192, where equal ranges took 61 with the same tiles; a chunk's start costs its warp 6 us without loads.)
 //
 // 32 / 8 heads of 128, us: 16 contexts of 32768 172 (6.2 TB/s), of 8192 57 (4.7), 64 of 1 .. 2048 37, one of 8192 14.  Of short work it is bound by
@@ -58,8 +59,7 @@ template <int D> constexpr int kTileOf = D == 64 ? 64 : 32;  // positions of a t
 inline int tile_of(int64_t dim) { return dim == 64 ? kTileOf<64> : kTileOf<128>; }
 constexpr int kEntry = 2;                    // what the change to another item costs a warp, in tiles
 constexpr int64_t kMaxContextHint = 1LL << 38;
-constexpr float kWeightLog2 = 14.0f;            // the largest weight of a head in FP16 is 2^14
-constexpr float kLeastScale = 8.0779357e-28f;   // 2^-90: scales of V below that, in units of the first tile's, count as that
+constexpr float kWeightLog2 = 14.0f;  // the largest weight of a head in FP16 is 2^14 .. 2^15
 
 // A stage: K rows, V rows (16-byte pieces xor-swizzled, so that eight rows of an ldmatrix lie on eight bank groups).
 template <int D>
@@ -154,16 +154,15 @@ __device__ __forceinline__ void store_dims(const PeerOut& out, int64_t row, int6
     }
   }
 }
-// Statistics in units of log2: merges (m, l) of b into a.
-__device__ __forceinline__ void merge_stats2(float& m_a, float& l_a, float& scale_a, float& scale_b, float m_b, float l_b) {
-  const float m = fmaxf(m_a, m_b);
-  scale_a = m_a == -INFINITY ? 0.0f : exp2_fast(m_a - m);
-  scale_b = m_b == -INFINITY ? 0.0f : exp2_fast(m_b - m);
-  l_a = l_a * scale_a + l_b * scale_b;
-  m_a = m;
+// The e of a scale that is not below 0 as 2^e * f, f in [1, 2), which takes its place; 0: 2^-infinity times 0, what is not finite: 2^0 times that.
+__device__ __forceinline__ float split_scale(float& scale) {
+  if (scale == 0.0f) return -INFINITY;
+  if (!(scale < INFINITY)) return 0.0f;
+  const bool small = scale < 7.8886091e-31f;  // 2^-100; below 2^-126 the exponent's bits do not tell it
+  const uint32_t bits = __float_as_uint(small ? scale * 1.2676506e30f : scale);
+  scale = __uint_as_float((bits & 0x7fffffu) | 0x3f800000u);
+  return static_cast<float>(static_cast<int>(bits >> 23) - (small ? 227 : 127));
 }
-// What the sum of the weights divides: nothing was attended to where it is 0.
-__device__ __forceinline__ float normalised(float acc, float l) { return l == 0.0f ? 0.0f : acc / l; }
 
 // ---- the line of tiles ---------------------------------------------------------------------------------------------------
 // Token by token, its KV heads; to each kEntry units and one for every tile of the context (one dead tile for an empty one).  Only the
@@ -276,7 +275,7 @@ template <bool SPARSE, typename Context> __device__ __forceinline__ int advance(
 }
 
 // Scratch of a grid of `warps`: slot 2 b + 1 is for the item that warp b begins and does not end, slot 2 b for one begun before
-// it.  Accumulators [slots][group * dim], running maxima and sums [slots][8] of each; and `shares`, which the warp that begins an item
+// it.  Results over the warp's positions [slots][group * dim], running maxima and sums [slots][8] of each; and `shares`, which the warp that begins an item
 // writes.  By item: that warp and how many warps have a part of it.  By warp, where there are more items than warps: the item that it begins and
 // does not end (there is one at most), and how many have a part of it, 1 if there is none.
 struct Partials {
@@ -301,7 +300,7 @@ kv8_attention_kernel(const __grid_constant__ Kv8Args a, const __grid_constant__ 
   constexpr bool CENTRED = SPLIT;    // FP32 results would see what an offset of the codes cancels
   extern __shared__ __align__(128) unsigned char ring[];
   __shared__ int64_t rows[TP];     // byte offsets of the rows that are fetched
-  __shared__ float4 per_row[TP];   // of a tile's positions: scale of K, log2 of that of V (-infinity: dead), one over it
+  __shared__ float4 per_row[TP];   // of a tile's positions: scale of K, 0 (-infinity: dead), significand and exponent of the scale of V
 
   pdl_launch_dependents();
   pdl_wait();  // q and the caches are the preceding kernels' output
@@ -482,17 +481,16 @@ kv8_attention_kernel(const __grid_constant__ Kv8Args a, const __grid_constant__ 
 #pragma unroll
     for (int e = 0; e < 2; ++e) s_zero[e] = -Codec<C>::kOffset * Codec<C>::kUnit * __shfl_sync(0xffffffffu, sum, (2 * quad + e) * 4);
   }
-  // Of heads 2 quad + {0, 1}: the running maximum of s + log2(scale of V), in units of log2 -- what makes the largest weight 2^14 --, and
-  // this thread's share of the sum of the softmax weights, which lack the scale.
-  float m_run[2], l_run[2];
+  // Of heads 2 quad + {0, 1}, in units of log2: the running maxima of s plus the exponent of the scale of V -- what makes the largest weight
+  // 2^kWeightLog2 or more -- and of s, and this thread's share of the sum of the softmax weights 2^(s - s_run).
+  float m_run[2], s_run[2], l_run[2];
   float o[NC][4];  // O^T: dims 16 c + 2 grow (+ 1 in the upper two), the same heads
 #pragma unroll
-  for (int e = 0; e < 2; ++e) m_run[e] = -INFINITY, l_run[e] = 0.0f;
+  for (int e = 0; e < 2; ++e) m_run[e] = s_run[e] = -INFINITY, l_run[e] = 0.0f;
 #pragma unroll
   for (int c = 0; c < NC; ++c)
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[c][e] = 0.0f;
-  float v_unit = 0.0f;  // scales of V are taken in units of the largest of the first tile
 
   // rows pb * 16 + lane % 16, pieces c + lane / 16 of an even c: offsets that the stage and pb are added to
   uint32_t at_piece[NC / 2];
@@ -501,21 +499,12 @@ kv8_attention_kernel(const __grid_constant__ Kv8Args a, const __grid_constant__ 
 
   for (int u = first; u < end; ++u) {
     fetch_next(stage == 0 ? NST - 1 : stage - 1, ks[NST - 1], vs[NST - 1]);
-    if (u == first) {
-      v_unit = vs[0][0];
-#pragma unroll
-      for (int r = 1; r < R; ++r) v_unit = fmaxf(v_unit, vs[0][r]);
-#pragma unroll
-      for (int sh = 16; sh > 0; sh >>= 1) v_unit = fmaxf(v_unit, __shfl_xor_sync(0xffffffffu, v_unit, sh));
-      if (!(v_unit > 1e-37f)) v_unit = 1.0f;
-    }
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const bool live = !(vs[0][r] < 0.0f);  // NaN is alive
-      float rel = __fdividef(vs[0][r], v_unit);
-      rel = rel < kLeastScale ? kLeastScale : rel;  // NaN passes
-      const float in_exponent = log2_fast(rel);
-      per_row[r * 32 + lane] = make_float4(ks[0][r] * k_lift, live ? in_exponent : -INFINITY, live ? exp2_fast(-in_exponent) : 0.0f, 0.0f);
+      float significand = live ? vs[0][r] : 0.0f;
+      const float exponent = split_scale(significand);
+      per_row[r * 32 + lane] = make_float4(ks[0][r] * k_lift, live ? 0.0f : -INFINITY, significand, exponent);
 #pragma unroll
       for (int s = 0; s < NST - 1; ++s) ks[s][r] = ks[s + 1][r], vs[s][r] = vs[s + 1][r];
     }
@@ -546,32 +535,34 @@ kv8_attention_kernel(const __grid_constant__ Kv8Args a, const __grid_constant__ 
           for (int n = 0; n < NQ; ++n) mma(sc[pb], k, qb[n][c + h]);
         }
       }
-    // ---- online softmax of the two heads.  With the scale of V in the exponent the weights have one running maximum; the sum
-    // takes the scale out again.
-    float mx[2] = {m_run[0], m_run[1]}, take_out[PB][2];
+    // ---- online softmax of the two heads
+    float mx[2] = {m_run[0], m_run[1]}, ms[2] = {s_run[0], s_run[1]};
 #pragma unroll
     for (int pb = 0; pb < PB; ++pb)
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
         const float4 f = per_row[pb * 16 + grow + r * 8];
-        take_out[pb][r] = f.z;
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           float& s = sc[pb][2 * r + e];
           s = fmaf(s, f.x * unit[e], f.y);
-          mx[e] = fmaxf(mx[e], s);
+          ms[e] = fmaxf(ms[e], s), mx[e] = fmaxf(mx[e], s + f.w);
         }
       }
-    float corr[2], from[2];
+    auto rebase = [&](float& run, float most) {  // to a maximum of all lanes; returns what the sums so far take
+#pragma unroll
+      for (int sh = 4; sh < 32; sh <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, sh));
+      const float by = most == -INFINITY ? 1.0f : exp2_fast(run - most);  // nothing yet
+      run = most;
+      return by;
+    };
+    float corr[2], from[2], sum_from[2];
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-#pragma unroll
-      for (int sh = 4; sh < 32; sh <<= 1) mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], sh));
-      from[e] = mx[e] == -INFINITY ? 0.0f : mx[e] - kWeightLog2;
-      corr[e] = exp2_fast(m_run[e] - mx[e]);
-      if (mx[e] == -INFINITY) corr[e] = 1.0f;  // nothing yet
-      m_run[e] = mx[e];
-      l_run[e] *= corr[e];
+      corr[e] = rebase(m_run[e], mx[e]);
+      l_run[e] *= rebase(s_run[e], ms[e]);
+      from[e] = m_run[e] == -INFINITY ? 0.0f : m_run[e] - kWeightLog2;
+      sum_from[e] = s_run[e] == -INFINITY ? 0.0f : s_run[e];
     }
     uint32_t wb[NQ][PB][2];  // w^T as B fragments: positions 16 pb + 2 quad + {0,1} (+ 8 in [1]), head grow
     float t_zero[2] = {0.0f, 0.0f};  // as s_zero: kOffset * the tile's weights
@@ -579,14 +570,19 @@ kv8_attention_kernel(const __grid_constant__ Kv8Args a, const __grid_constant__ 
     for (int pb = 0; pb < PB; ++pb)
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        const float x0 = exp2_fast(sc[pb][2 * r] - from[0]), x1 = exp2_fast(sc[pb][2 * r + 1] - from[1]);
-        l_run[0] = fmaf(x0, take_out[pb][r], l_run[0]), l_run[1] = fmaf(x1, take_out[pb][r], l_run[1]);
-        const __half2 hi = __floats2half2_rn(x0, x1);
+        const float4 f = per_row[pb * 16 + grow + r * 8];
+        float x[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float s = sc[pb][2 * r + e];
+          x[e] = exp2_fast(s + f.w - from[e]) * f.z, l_run[e] += exp2_fast(s - sum_from[e]);
+        }
+        const __half2 hi = __floats2half2_rn(x[0], x[1]);
         wb[0][pb][r] = transpose8x8(*reinterpret_cast<const uint32_t*>(&hi));
         if constexpr (SPLIT || Codec<C>::kOffset != 0.0f) {
-          const float2 f = __half22float2(hi);
-          if constexpr (SPLIT) wb[NQ - 1][pb][r] = transpose8x8(Mma16816<__half>::pack(x0 - f.x, x1 - f.y));
-          else t_zero[0] += f.x, t_zero[1] += f.y;
+          const float2 h = __half22float2(hi);
+          if constexpr (SPLIT) wb[NQ - 1][pb][r] = transpose8x8(Mma16816<__half>::pack(x[0] - h.x, x[1] - h.y));
+          else t_zero[0] += h.x, t_zero[1] += h.y;
         }
       }
     if constexpr (!CENTRED && Codec<C>::kOffset != 0.0f) {
@@ -632,6 +628,7 @@ kv8_attention_kernel(const __grid_constant__ Kv8Args a, const __grid_constant__ 
 
   // ---- the result, or this warp's share of it
   const bool whole = first == 0 && end == cur.tiles;
+  constexpr float kValueUnit = CENTRED ? 1.0f : 1.0f / Codec<C>::kUnit;
   const Partials part(a.scratch, gridDim.x, G * D);
   const size_t slot = 2 * static_cast<size_t>(blockIdx.x) + (first == 0 ? 1 : 0);
   if (first == 0 && lane == 0) {  // an item that others go on with ends cur.tiles - end units behind this warp's share
@@ -646,18 +643,18 @@ kv8_attention_kernel(const __grid_constant__ Kv8Args a, const __grid_constant__ 
     for (int sh = 4; sh < 32; sh <<= 1) l_run[e] += __shfl_xor_sync(0xffffffffu, l_run[e], sh);
     const int head = quad * 2 + e;
     if (head >= G) continue;
+    // o / l times 2^(m_run - kWeightLog2 - s_run), in two halves, which keeps what is on the way in range
+    const float each = l_run[e] == 0.0f ? 0.0f : 1.0f / l_run[e] * kValueUnit;
+    const float half = m_run[e] == -INFINITY ? 0.0f : exp2_fast(0.5f * (m_run[e] - kWeightLog2 - s_run[e]));
+    auto value = [&](int c, int i) { return o[c][e + 2 * i] * half * each * half; };
     if (whole) {
-      // o / l, then the units, which keeps what is on the way in range
-      const float each = l_run[e] == 0.0f ? 0.0f : 1.0f / l_run[e];
-      store_dims<SPLIT>(out, token, static_cast<int64_t>(kvh * G + head) * D + 2 * grow, a.dtype, a.paired,
-                        [&](int c, int i) { return o[c][e + 2 * i] * each / (CENTRED ? 1.0f : Codec<C>::kUnit) * v_unit; }, std::integral_constant<int, NC>());
+      store_dims<SPLIT>(out, token, static_cast<int64_t>(kvh * G + head) * D + 2 * grow, a.dtype, a.paired, value, std::integral_constant<int, NC>());
     } else {
-      const float back = v_unit / (CENTRED ? 1.0f : Codec<C>::kUnit);
       float* to = part.acc + (slot * G + head) * D + 2 * grow;
 #pragma unroll
-      for (int c = 0; c < NC; ++c) *reinterpret_cast<float2*>(to + c * 16) = make_float2(o[c][e] * back, o[c][e + 2] * back);
+      for (int c = 0; c < NC; ++c) *reinterpret_cast<float2*>(to + c * 16) = make_float2(value(c, 0), value(c, 1));
       if (grow == 0) {
-        part.m[slot * kMaxGroup + head] = m_run[e];
+        part.m[slot * kMaxGroup + head] = s_run[e];
         part.l[slot * kMaxGroup + head] = l_run[e];
       }
     }
@@ -667,13 +664,41 @@ kv8_attention_kernel(const __grid_constant__ Kv8Args a, const __grid_constant__ 
   }
 }
 
+// Of one head: the result of some positions, and the sum of their softmax weights, l, in units of 2^m.
+struct Part {
+  float4 value;
+  float m, l;
+};
+// Adds N parts to a sum of parts.  The values enter with their shares of all weights, so that they pass no range that the result does not; a
+// share has its power of two in two halves, as a large value counts with one below 2^-126 where all others are as small.
+template <int N> __device__ __forceinline__ void add_parts(Part& sum, const Part (&p)[N]) {
+  float m = sum.m;
+#pragma unroll
+  for (int i = 0; i < N; ++i) m = fmaxf(m, p[i].m);
+  const float from = m == -INFINITY ? 0.0f : m, had = exp2_fast(0.5f * (sum.m - from));
+  float half[N], l = sum.l * had * had;
+#pragma unroll
+  for (int i = 0; i < N; ++i) half[i] = exp2_fast(0.5f * (p[i].m - from)), l += p[i].l * half[i] * half[i];
+  const float per = l == 0.0f ? 0.0f : 1.0f / l;
+  float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  auto add = [&](const Part& part, float h) {
+    const float share = part.l * per * h;
+    v.x = fmaf(part.value.x * h, share, v.x), v.y = fmaf(part.value.y * h, share, v.y);
+    v.z = fmaf(part.value.z * h, share, v.z), v.w = fmaf(part.value.w * h, share, v.w);
+  };
+  add(sum, had);
+#pragma unroll
+  for (int i = 0; i < N; ++i) add(p[i], half[i]);
+  sum = {v, m, l};
+}
+
 // Adds the parts of an item, one for each entry of `shares`: L lanes of four values each to a CTA, the THREADS / L groups of them every so
-// many parts; the groups' sums meet in shared memory.  Always in the same order.  L: a warp where there are few items, so that many CTAs
+// many parts, two at a time; the groups' sums meet in shared memory.  Always in the same order.  L: a warp where there are few items, so that many CTAs
 // share an item; else what the group * dim values take, at most all threads.
 template <int L, int THREADS>
 __global__ void __launch_bounds__(THREADS)
 kv8_attention_merge_kernel(const __grid_constant__ Kv8Args a, const __grid_constant__ PeerOut out, int dim, int grid) {
-  constexpr int kGroups = THREADS / L;
+  constexpr int kGroups = THREADS / L, N = 2;
   __shared__ float4 accs[kGroups][L];
   __shared__ float ms[kGroups][L], ls[kGroups][L];
   pdl_launch_dependents();
@@ -686,33 +711,43 @@ kv8_attention_merge_kernel(const __grid_constant__ Kv8Args a, const __grid_const
   const int item = a.by_warp ? share.x : blockIdx.x, begins = a.by_warp ? blockIdx.x : share.x;
   const bool some = at < all;
   const int head = some ? at / dim : 0;
-  float m = -INFINITY, l = 0.0f;
-  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  auto add = [&](const float4& v, float mv, float lv) {
-    float sa, sb;
-    merge_stats2(m, l, sa, sb, mv, lv);
-    acc.x = acc.x * sa + v.x * sb, acc.y = acc.y * sa + v.y * sb;
-    acc.z = acc.z * sa + v.z * sb, acc.w = acc.w * sa + v.w * sb;
-  };
-#pragma unroll 8
-  for (int i = group; i < share.y; i += kGroups) {
-    const size_t slot = 2 * static_cast<size_t>(begins + i) + (i == 0 ? 1 : 0);
-    const float4 v = some ? __ldcg(reinterpret_cast<const float4*>(part.acc + slot * all + at)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    add(v, __ldcg(part.m + slot * kMaxGroup + head), __ldcg(part.l + slot * kMaxGroup + head));
+  const Part none = {make_float4(0.0f, 0.0f, 0.0f, 0.0f), -INFINITY, 0.0f};
+  Part sum = none, p[N];
+#pragma unroll 1
+  for (int first = group; first < share.y; first += kGroups * N) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int i = first + k * kGroups;
+      const size_t slot = 2 * static_cast<size_t>(begins + i) + (i == 0 ? 1 : 0);
+      p[k] = none;
+      if (some && i < share.y) {
+        p[k].value = __ldcg(reinterpret_cast<const float4*>(part.acc + slot * all + at));
+        p[k].m = __ldcg(part.m + slot * kMaxGroup + head), p[k].l = __ldcg(part.l + slot * kMaxGroup + head);
+      }
+    }
+    add_parts(sum, p);
   }
   if constexpr (kGroups > 1) {
-    accs[group][lane] = acc, ms[group][lane] = m, ls[group][lane] = l;
+    accs[group][lane] = sum.value, ms[group][lane] = sum.m, ls[group][lane] = sum.l;
     __syncthreads();
     if (group != 0) return;
-    for (int w = 1; w < kGroups; ++w) add(accs[w][lane], ms[w][lane], ls[w][lane]);
+    constexpr int kRest = kGroups < 8 ? kGroups : 8;
+    sum = none;
+#pragma unroll
+    for (int first = 0; first < kGroups; first += kRest) {
+      Part q[kRest];
+#pragma unroll
+      for (int k = 0; k < kRest; ++k) q[k] = {accs[first + k][lane], ms[first + k][lane], ls[first + k][lane]};
+      add_parts(sum, q);
+    }
   }
   if (!some) return;
   const int token = item / a.kv_heads, kvh = item - token * a.kv_heads;
   const int64_t col = static_cast<int64_t>(kvh) * all + at;
-  store_from_f32(out, token, col, normalised(acc.x, l), a.dtype);
-  store_from_f32(out, token, col + 1, normalised(acc.y, l), a.dtype);
-  store_from_f32(out, token, col + 2, normalised(acc.z, l), a.dtype);
-  store_from_f32(out, token, col + 3, normalised(acc.w, l), a.dtype);
+  store_from_f32(out, token, col, sum.value.x, a.dtype);
+  store_from_f32(out, token, col + 1, sum.value.y, a.dtype);
+  store_from_f32(out, token, col + 2, sum.value.z, a.dtype);
+  store_from_f32(out, token, col + 3, sum.value.w, a.dtype);
 }
 
 // ---- host --------------------------------------------------------------------------------------------------------------
@@ -742,8 +777,8 @@ int launch_kv8(Kv8Args a, const PeerOut& out, int warps, cudaStream_t s) {
     return launch_opts(kernel, dim3(static_cast<unsigned>(entries), static_cast<unsigned>((lanes + l - 1) / l)), dim3(threads), 0, s, 1u, true, a, out, D,
                        warps);
   };
-  // at most one CTA to an SM: of 512 threads, sixteen parts at once (one context of 8192, 130 parts a head: 15.9 -> 13.9 us; in more CTAs than
-  // that 256 threads are faster, 57.5 against 58.9 for 16 of them)
+  // at most one CTA to an SM: of 512 threads, sixteen groups (one context of 8192, 130 parts a head: 15.9 -> 13.9 us when both had one part at a
+  // time; in more CTAs than that 256 threads are faster, 57.5 against 58.9 for 16 of them)
   if (entries * ((lanes + 31) / 32) <= sm_count()) return merge(kv8_attention_merge_kernel<32, 512>, 32, 512);
   if (entries <= sm_count() || lanes <= 32) return merge(kv8_attention_merge_kernel<32, 256>, 32, 256);
   return lanes <= 128 ? merge(kv8_attention_merge_kernel<128, 256>, 128, 256) : merge(kv8_attention_merge_kernel<256, 256>, 256, 256);

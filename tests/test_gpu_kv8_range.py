@@ -35,3 +35,47 @@ def test_q_of_any_size(codes, dtype, exponents):
         _reads(q.to(dtype), cache, pos, table, seq, dtype)
         q[:, 1::2] *= 2.0 ** -8  # heads of a group that differ
         _reads(q.to(dtype), cache, pos, table, seq, dtype)
+
+
+def _scaled(cache, table, seq, rows):
+    """`rows`: {slice of a context's pages: exponent, or None for blocks of zeros}; in all contexts."""
+    scale = cache["v_scale"]
+    for part, exponent in rows.items():
+        at = table[seq][:, part].flatten()
+        if exponent is None:
+            scale[at] = 0
+            cache["v"].view(torch.uint8)[at] = 0
+        else:
+            scale[at] = torch.ldexp(scale[at], torch.tensor(exponent))
+
+
+FAR = {
+    "first far below": {slice(0, 2): -120, slice(2, None): 8}, "first far above": {slice(0, 2): 30, slice(2, None): -100},
+    "one far below": {slice(7, 8): -115}, "one far above": {slice(9, 10): 100}, "last far above": {slice(-1, None): 118},
+    "first zero, tiny behind": {slice(0, 3): None, slice(3, None): -110}, "one zero": {slice(20, 21): None}, "all zero": {slice(0, None): None},
+    "all tiny": {slice(0, None): -116}, "all large": {slice(0, None): 118},
+    "steps": {slice(i, i + 1): 100 - 6 * i for i in range(34)}, "steps up": {slice(i, i + 1): -100 + 6 * i for i in range(34)},
+}
+
+
+@pytest.mark.parametrize("codes,dtype", [(INT8, BF16), (E4M3, BF16), (INT8, F32), (E4M3, F32)])
+@pytest.mark.parametrize("rows", FAR.values(), ids=FAR.keys())
+def test_scales_of_v_far_from_each_other(codes, dtype, rows):
+    """Blocks whose V is larger or smaller by up to 2^230 than in the pages in front of them, or nothing: results of ordinary scores, and of
+    scores so far apart that the small blocks have the weight."""
+    for dim, spread, top in ((128, 1.0, 1.0), (64, 300.0, 1.0), (256, 40.0, 1.0)):
+        cache, pos, table, seq = _attend_inputs((6, 2), dim, 16, [540, 300, 543], codes, seed=33)
+        _scaled(cache, table, seq, rows)
+        cache["k_scale"] *= spread / 10
+        q = (torch.randn(3, 6, dim, generator=_gen(33)) * top).to(dtype)
+        _reads(q, cache, pos, table, seq, dtype, "HND")
+
+
+@pytest.mark.parametrize("codes", [INT8, E4M3])
+def test_scales_of_zero_over_codes_that_are_not(codes):
+    """A scale of 0 makes its block 0, whatever the codes are: alone in a context, in front of others and behind them."""
+    cache, pos, table, seq = _attend_inputs((8, 2), 128, 16, [540, 300, 20], codes, seed=34)
+    cache["v_scale"][table[seq[0], 3:20]] = 0
+    cache["v_scale"][table[seq[1], :4]] = 0
+    cache["v_scale"][table[seq[2]]] = 0
+    _reads(torch.randn(3, 8, 128, generator=_gen(34)).half(), cache, pos, table, seq, F16)
