@@ -1,4 +1,9 @@
 // Status codes, error text and the device gate of the C ABI.
+#include <exception>
+#include <map>
+#include <mutex>
+#include <utility>
+
 #include "common.cuh"
 
 namespace xdk {
@@ -14,6 +19,24 @@ int note_launch(cudaError_t err) {
   g_last_cuda_error = static_cast<int>(err);
   (void)cudaGetLastError();  // clear the sticky-free launch error so later calls start clean
   return XDK_ERR_LAUNCH;
+}
+
+int allow_smem(const void* kernel, size_t bytes) {
+  static std::mutex lock;
+  static std::map<std::pair<int, const void*>, size_t> most;  // of this process, by device and kernel
+  int dev = -1;
+  if (const cudaError_t err = cudaGetDevice(&dev)) return note_launch(err);
+  try {
+    const std::lock_guard<std::mutex> held(lock);
+    size_t& known = most[{dev, kernel}];
+    const size_t limit = bytes > known ? bytes : known;
+    if (const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(limit)))
+      return note_launch(err);
+    known = limit;
+  } catch (const std::exception&) {  // none may pass the C entry points
+    return note_launch(cudaErrorMemoryAllocation);
+  }
+  return XDK_OK;
 }
 
 int require_sm100() {

@@ -15,6 +15,9 @@ namespace xdk {
 
 // Records the runtime's error for xdk_last_cuda_error() and maps it to a status.
 int note_launch(cudaError_t err);
+// Lets `kernel` have `bytes` of dynamic shared memory on the current device, before a launch with that much.  The limit belongs to the function
+// and so to all host threads: it is only ever raised, so that no call takes from another what that is about to launch with.
+int allow_smem(const void* kernel, size_t bytes);
 // XDK_OK when the device current to this thread is compute capability 10.x (cached per device).
 int require_sm100();
 

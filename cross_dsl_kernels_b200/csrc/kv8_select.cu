@@ -226,8 +226,7 @@ template <typename T>
 int dispatch_select(int64_t d, const SelectArgs& a, dim3 grid, size_t smem, cudaStream_t s) {
   auto run = [&](auto kernel) {
     if (smem > 32 * 1024) {  // with the 9 KB that it has statically, beyond what a launch gets unasked
-      const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-      if (err != cudaSuccess) return note_launch(err);
+      if (int st = allow_smem(reinterpret_cast<const void*>(kernel), smem)) return st;
     }
     return launch_dependent(kernel, grid, dim3(kSelThreads), smem, s, a);
   };

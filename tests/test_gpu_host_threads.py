@@ -1,0 +1,51 @@
+"""Two host threads that call an op at the same time, with sizes that take different amounts of shared memory."""
+
+from __future__ import annotations
+
+import threading
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def _side_by_side(calls, rounds=4000):
+    """Each of `calls` in a thread and on a stream of its own, over and over; every result is that of the call alone."""
+    alone = [call() for call in calls]
+    torch.cuda.synchronize()
+    wrong, start = [], threading.Barrier(len(calls))
+
+    def run(call, want):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                start.wait()
+                for i in range(rounds):
+                    got = call()
+                    if i % 500 == 499 and not torch.equal(got, want):
+                        wrong.append("another result")
+        except Exception as error:  # a thread's own would be lost
+            wrong.append(repr(error))
+
+    threads = [threading.Thread(target=run, args=pair) for pair in zip(calls, alone)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not wrong, wrong[0]
+
+
+def test_selections_from_tables_of_different_widths():
+    from cross_dsl_kernels_b200 import kv8
+
+    def call(width):
+        g = torch.Generator(device="cuda").manual_seed(width)
+        cache = kv8.PagedKV8Cache.empty(width, 1, 1, 64)
+        cache.k_mean.copy_(torch.randint(-60, 61, cache.k_mean.shape, generator=g, device="cuda", dtype=torch.int8))
+        cache.k_scale.fill_(1.0)
+        q = torch.randn(1, 2, 64, generator=g, device="cuda")
+        index = (torch.tensor([width - 1], device="cuda"), torch.randperm(width, generator=g, device="cuda")[None], torch.zeros(1, dtype=torch.int64, device="cuda"))
+        return lambda: kv8.select_kv8_pages(q, cache, *index, top_pages=9)
+
+    _side_by_side([call(51200), call(9000)])
