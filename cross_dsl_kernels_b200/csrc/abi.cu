@@ -73,9 +73,18 @@ bool encode_tiled(CUtensorMap* map, CUtensorMapDataType type, int rank, const vo
   }
   const cuuint32_t elem_strides[5] = {1, 1, 1, 1, 1};
   if (rank < 1 || rank > 5) return false;
-  return encode(map, type, static_cast<cuuint32_t>(rank), const_cast<void*>(base), dims, strides_bytes, box, elem_strides, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                swizzle128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
-                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  auto run = [&]() {
+    return encode(map, type, static_cast<cuuint32_t>(rank), const_cast<void*>(base), dims, strides_bytes, box, elem_strides, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  swizzle128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  CUresult result = run();
+  if (result == CUDA_ERROR_INVALID_CONTEXT) {  // a host thread that has called nothing of the runtime yet has no context
+    int dev = -1;
+    if (cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess) result = run();
+    (void)cudaGetLastError();
+  }
+  return result == CUDA_SUCCESS;
 }
 
 bool encode_tiled_2d(CUtensorMap* map, CUtensorMapDataType type, const void* base, const cuuint64_t* dims,

@@ -49,3 +49,30 @@ def test_selections_from_tables_of_different_widths():
         return lambda: kv8.select_kv8_pages(q, cache, *index, top_pages=9)
 
     _side_by_side([call(51200), call(9000)])
+
+
+@pytest.mark.parametrize("m", [1, 4, 16])
+def test_first_call_of_a_thread(m):
+    """A thread that has not used the GPU before: the same bits as in the main thread, for projections of each kind."""
+    from cross_dsl_kernels_b200.ops import decode_linear
+    from cross_dsl_kernels_b200.w4a16 import w4a16_linear
+    g = torch.Generator(device="cuda").manual_seed(m)
+    x, w = (torch.randn(*shape, generator=g, device="cuda") for shape in ((m, 1024), (1024, 4096)))
+    packed = torch.randint(0, 256, (4096, 512), generator=g, device="cuda", dtype=torch.uint8)
+    scales, half = torch.rand(4096, 8, generator=g, device="cuda").half(), x.half()
+    for call in (lambda: w4a16_linear(half, packed, scales, None, group_size=128), lambda: decode_linear(x, w, None, weight_layout="KN"),
+                 lambda: decode_linear(x, w.view(4096, 1024), None, weight_layout="NK")):
+        want, got = call(), []
+
+        def run():
+            try:
+                got.append(call())
+            except Exception as error:  # a thread's own would be lost
+                got.append(error)
+
+        thread = threading.Thread(target=run)
+        thread.start()
+        thread.join()
+        torch.cuda.synchronize()
+        assert isinstance(got[0], torch.Tensor), got[0]
+        assert torch.equal(got[0], want)
