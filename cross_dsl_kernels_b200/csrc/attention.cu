@@ -848,8 +848,7 @@ int launch_attention_cluster(const void* q, const void* kc, const void* vc, cons
     if (smem < acc_bytes) smem = acc_bytes;
   }
   if (smem > 48 * 1024) {
-    cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-    if (err != cudaSuccess) return note_launch(err);
+    if (int st = allow_smem(reinterpret_cast<const void*>(kernel), smem)) return st;
   }
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;

@@ -535,9 +535,7 @@ template <int MT, int BNCOLS> constexpr size_t smem_bytes() { return (2 * MT * k
 
 template <typename Kernel>
 int launch_gemv(Kernel kernel, size_t smem, const GemvArgs& a, int bn, int splits, cudaStream_t stream) {
-  // Opt in to > 48 KB of dynamic shared memory (a per-function attribute; cheap to repeat).
-  cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-  if (err != cudaSuccess) return note_launch(err);
+  if (int st = allow_smem(reinterpret_cast<const void*>(kernel), smem)) return st;
   dim3 grid((a.n + bn - 1) / bn, splits, (a.m + 15) / 16);
   return launch(kernel, grid, dim3(kThreads), smem, stream, static_cast<unsigned>(splits), a);
 }
@@ -592,13 +590,11 @@ int launch_tile_stream(const float* x, const float* w, const float* bias, const 
   int st;
   if (nk) {
     auto kernel = gemv_stream_kernel<MT, true>;
-    cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-    if (err != cudaSuccess) return note_launch(err);
+    if (int st = allow_smem(reinterpret_cast<const void*>(kernel), smem)) return st;
     st = launch(kernel, dim3(a.ctas), dim3(kTileThreads), smem, stream, 1u, a, wmap, xmap);
   } else {
     auto kernel = gemv_stream_kernel<MT, false>;
-    cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-    if (err != cudaSuccess) return note_launch(err);
+    if (int st = allow_smem(reinterpret_cast<const void*>(kernel), smem)) return st;
     st = launch(kernel, dim3(a.ctas), dim3(kTileThreads), smem, stream, 1u, a, wmap, xmap);
   }
   if (st != XDK_OK) return st;

@@ -308,8 +308,7 @@ int launch_mma(const MmaArgs& a, int ctas, int ranks, int blocks, cudaStream_t s
   constexpr size_t smem = Ring<NK, G>::bytes(MR);
   static_assert(smem <= 227 * 1024, "one CTA per SM");
   auto kernel = gemv_mma_kernel<NK, MR, G>;
-  cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-  if (err != cudaSuccess) return note_launch(err);
+  if (int st = allow_smem(reinterpret_cast<const void*>(kernel), smem)) return st;
   return launch_opts(kernel, dim3(ctas, ranks, blocks), dim3(kThreads), smem, stream, static_cast<unsigned>(ranks),
                      (call_flags() & XDK_DEPENDENT_LAUNCH) != 0, a);
 }

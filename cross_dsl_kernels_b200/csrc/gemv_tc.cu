@@ -546,7 +546,7 @@ int resident_clusters(int parts) {
     attr.val.clusterDim.x = 1, attr.val.clusterDim.y = static_cast<unsigned>(parts), attr.val.clusterDim.z = 1;
     cfg.gridDim = dim3(sms / parts, parts), cfg.blockDim = dim3(kThreads), cfg.dynamicSmemBytes = smem, cfg.attrs = &attr, cfg.numAttrs = 1;
     int n = 0;
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) == cudaSuccess &&
+    if (allow_smem(reinterpret_cast<const void*>(kernel), smem) == XDK_OK &&
         cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) == cudaSuccess && n > 0)
       fit = n < sms / parts ? n : sms / parts;
   }
@@ -632,8 +632,7 @@ int launch_tc(const float* x, const float* w, const float* bias, const PeerOut& 
   const cuuint32_t xbox[4] = {kStepK, static_cast<cuuint32_t>(a.split), 1, 16};
   if (!encode_tiled(&xmap, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, x, xdims, xstrides, xbox, false)) return XDK_ERR_LAUNCH;
   auto kernel = gemv_tc_kernel<NK>;
-  cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-  if (err != cudaSuccess) return note_launch(err);
+  if (int st = allow_smem(reinterpret_cast<const void*>(kernel), smem)) return st;
   return launch(kernel, dim3(a.ctas, a.kparts), dim3(kThreads), smem, stream, static_cast<unsigned>(a.kparts), a, wmaps[0],
                 wmaps[1], wmaps[2], wmaps[3], xmap);
 }

@@ -471,8 +471,7 @@ int launch_stream(const W4Args& a, cudaStream_t stream) {
     }
   }
   auto kernel = w4a16_stream_kernel<MR>;
-  cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-  if (err != cudaSuccess) return note_launch(err);
+  if (int st = allow_smem(reinterpret_cast<const void*>(kernel), smem)) return st;
   cudaLaunchConfig_t cfg = {};
   cfg.blockDim = dim3(kStreamThreads);
   cfg.dynamicSmemBytes = smem;
@@ -938,8 +937,7 @@ int launch_umma(const W4Args& a, bool dependent, cudaStream_t stream) {
     const cuuint32_t xbox[2] = {kUStepK, 16};
     if (!encode_tiled(&xmap, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, a.x, xdims, xstrides, xbox, false)) return XDK_ERR_LAUNCH;
   }
-  cudaError_t err = cudaFuncSetAttribute(w4a16_umma_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-  if (err != cudaSuccess) return note_launch(err);
+  if (int st = allow_smem(reinterpret_cast<const void*>(w4a16_umma_kernel), smem)) return st;
   return launch_opts(w4a16_umma_kernel, dim3(plan.ctas), dim3(kUThreads), smem, stream, 1u, dependent, a, plan, wmap, smap, xmap);
 }
 
@@ -1146,12 +1144,11 @@ template <int CHUNKS, int CTAS>
 int launch_mma(W4Args a, bool dependent, cudaStream_t stream) {
   const size_t xbytes = (static_cast<size_t>(a.m) * (a.k * 2 + 16) + 127) & ~static_cast<size_t>(127);
   const size_t smem = xbytes + 2 * static_cast<size_t>(kWarps) * 32 * 4 * sizeof(float);
-  cudaError_t err = cudaFuncSetAttribute(w4a16_mma_kernel<CHUNKS, CTAS>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-  if (err != cudaSuccess) return note_launch(err);
+  if (int st = allow_smem(reinterpret_cast<const void*>(w4a16_mma_kernel<CHUNKS, CTAS>), smem)) return st;
   // one wave: as many CTAs as the device holds at once (two per SM unless x takes more than half the shared memory);
   // a grid of a few CTAs more than that ran as two waves and took twice the time
   int resident = 0;
-  err = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, w4a16_mma_kernel<CHUNKS, CTAS>, kThreads, smem);
+  const cudaError_t err = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, w4a16_mma_kernel<CHUNKS, CTAS>, kThreads, smem);
   if (err != cudaSuccess) return note_launch(err);
   if (resident < 1) return XDK_ERR_LIMIT;
   const int groups = (a.n + 15) / 16;
@@ -1411,7 +1408,7 @@ int rx_resident_clusters(int ranks) {  // the same for every variant: one CTA pe
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
   int n = known[dev][ranks].load(std::memory_order_relaxed);
   if (n > 0) return n;
-  if (cudaFuncSetAttribute(w4a16_rx_kernel<2>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRxSmem) != cudaSuccess) return 0;
+  if (allow_smem(reinterpret_cast<const void*>(w4a16_rx_kernel<2>), kRxSmem) != XDK_OK) return 0;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(sm_count() / ranks, ranks);
   cfg.blockDim = dim3(kRxWarps * 32);
@@ -1432,8 +1429,7 @@ int rx_resident_clusters(int ranks) {  // the same for every variant: one CTA pe
 template <int MR>
 int launch_rx(const W4Args& a, bool dependent, bool one_wave, cudaStream_t stream) {
   RxPlan p = {};
-  cudaError_t err = cudaFuncSetAttribute(w4a16_rx_kernel<MR>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRxSmem);
-  if (err != cudaSuccess) return note_launch(err);
+  if (int st = allow_smem(reinterpret_cast<const void*>(w4a16_rx_kernel<MR>), kRxSmem)) return st;
   const int sms = sm_count();
   p.slices = (a.k + kRxSliceK - 1) / kRxSliceK;
   p.groups = (a.n + 15) / 16;
@@ -1477,8 +1473,7 @@ template <int MT, int CW>
 int launch_simt(W4Args a, cudaStream_t stream) {
   const size_t smem = static_cast<size_t>(MT) * a.k * sizeof(__half);
   auto kernel = w4a16_simt_kernel<MT, CW>;
-  cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-  if (err != cudaSuccess) return note_launch(err);
+  if (int st = allow_smem(reinterpret_cast<const void*>(kernel), smem)) return st;
   a.col_groups = (a.n + kWarps * CW - 1) / (kWarps * CW);
   const int max_ctas = 4 * sm_count();
   a.groups_per_cta = (a.col_groups + max_ctas - 1) / max_ctas;

@@ -76,3 +76,18 @@ def test_first_call_of_a_thread(m):
         torch.cuda.synchronize()
         assert isinstance(got[0], torch.Tensor), got[0]
         assert torch.equal(got[0], want)
+
+
+@pytest.mark.parametrize("one,two", [((1, 96000), (1, 1600)), ((8, 8192), (8, 2048)), ((16, 6080), (16, 160))])
+def test_projections_of_different_depths(one, two):
+    """x stays in shared memory, as much as there is of it."""
+    from cross_dsl_kernels_b200.w4a16 import w4a16_linear
+
+    def call(m, k):
+        g = torch.Generator(device="cuda").manual_seed(k)
+        x = torch.randn(m, k, generator=g, device="cuda").half()
+        packed = torch.randint(0, 256, (64, k // 2), generator=g, device="cuda", dtype=torch.uint8)
+        scales = torch.rand(64, k // 32, generator=g, device="cuda").half()
+        return lambda: w4a16_linear(x, packed, scales, None, group_size=32)
+
+    _side_by_side([call(*one), call(*two)])
