@@ -66,14 +66,14 @@ kv8_select_kernel(const __grid_constant__ SelectArgs a) {
   int32_t* out = a.pages + (static_cast<int64_t>(token) * a.kv_heads + kvh) * a.top_pages;
   const int64_t pos = a.positions[token];
   if (pos < 0) {
-    for (int i = tid; i < a.top_pages; i += kSelThreads) out[i] = -1;
+    for (unsigned i = tid; i < static_cast<unsigned>(a.top_pages); i += kSelThreads) out[i] = -1;  // unsigned: the last step may pass 2^31
     return;
   }
   const int64_t at_page = pos / a.page_size;
   const int last = static_cast<int>(at_page < a.max_pages ? at_page : a.max_pages - 1);
   const int want = a.top_pages - 1;  // of the pages in front of the last one
   if (last <= want) {
-    for (int i = tid; i < a.top_pages; i += kSelThreads) out[i] = i <= last ? i : -1;
+    for (unsigned i = tid; i < static_cast<unsigned>(a.top_pages); i += kSelThreads) out[i] = i <= static_cast<unsigned>(last) ? static_cast<int>(i) : -1;
     return;
   }
   if (want == 0) {

@@ -79,3 +79,20 @@ def test_scales_of_zero_over_codes_that_are_not(codes):
     cache["v_scale"][table[seq[1], :4]] = 0
     cache["v_scale"][table[seq[2]]] = 0
     _reads(torch.randn(3, 8, 128, generator=_gen(34)).half(), cache, pos, table, seq, F16)
+
+
+@pytest.mark.parametrize("position", [-1, 100])
+def test_selection_of_as_many_pages_as_there_can_be(position):
+    """The largest top_pages: what stands behind the context's pages is -1 up to the end."""
+    from cross_dsl_kernels_b200.kv8 import select_kv8_pages
+    if torch.cuda.mem_get_info()[0] < 12 << 30:
+        pytest.skip("needs 12 GB of device memory")
+    cache, pos, table, seq = _attend_inputs((2, 1), 64, 16, [100], INT8, seed=35)
+    pos[0] = position
+    top = 2 ** 31 - 1
+    got = select_kv8_pages(torch.ones(1, 2, 64, device="cuda"), _on_gpu(cache, "NHD"), *(t.cuda() for t in (pos, table, seq)), top_pages=top)
+    assert got.shape == (1, 1, top)
+    pages = 0 if position < 0 else position // 16 + 1
+    assert got[0, 0, :pages].tolist() == list(range(pages))
+    for part in got[0, 0, pages:].split(1 << 29):
+        assert bool((part == -1).all())
