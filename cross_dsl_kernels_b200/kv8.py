@@ -41,8 +41,8 @@ class PagedKV8Cache:
 
     ``k``, ``v``: int8 or float8_e4m3fn, [pages, page_size, kv_heads, head_dim] ("NHD") or [pages, kv_heads, page_size, head_dim]
     ("HND"); ``k_scale``, ``v_scale``: float32 [pages, kv_heads], a value is code * scale, and no scale is negative; ``k_mean``: int8 [pages, kv_heads,
-    head_dim], the mean key of each full block in units of its scale (e4m3: of its scale * 448 / 127), or None for a cache from
-    which no pages are selected."""
+    head_dim], the mean key of each full block in units of its scale (e4m3: of its scale * 448 / 127), both as the call left them that
+    wrote the block's last position, or None for a cache from which no pages are selected."""
 
     k: torch.Tensor
     v: torch.Tensor
@@ -142,7 +142,8 @@ def rope_gqa_paged_kv8_append(q, k, v, cos, sin, positions, page_table, sequence
 
     The arguments are those of :func:`cross_dsl_kernels_b200.ops.rope_gqa_paged_kv_append`.  A block's scale is the largest
     |value| it was given since its first position was written, / 127 (int8) or 448 (e4m3); where a call makes it grow, the block's
-    other codes are rounded to the new scale.  A block whose last position is written gets its mean key.  Tokens may come in any order, several
+    other codes are rounded to the new scale.  A block whose last position is written gets its mean key; a call that writes others
+    of its positions anew leaves that as it is, until the last one is written again, too.  Tokens may come in any order, several
     for one page, and of several for one slot the last one counts.  A token with a position below 0 is padding: nothing is written
     for it, and its row of the result is 0.  A value that is not finite makes its block read as NaN until the page is begun anew."""
     done = _native.host().kv8_append(q, k, v, cos, sin, positions, page_table, sequence_ids, *_parts(cache), rope_dim, interleaved,

@@ -314,7 +314,8 @@ XDK_API int xdk_swiglu_peer(const void* upgate, const xdk_peer_out* out_dst, int
  *     before = 0 if row 0 is in W, else its scale; scale = max(before, max |x| of W * (1 / top))
  *     rows in W: code = round(x / scale), half to even (two tokens for one slot: the one with the larger index); the other rows, if row 0
  *     is not in W and the scale grew: code = round(code * (before / scale)).
- *     If the last row is in W, the mean of the block's codes as int8, in units of scale, or of scale * 448 / 127 for e4m3.
+ *     If the last row is in W, the mean of the block's codes as int8, in units of scale, or of scale * 448 / 127 for e4m3; else it
+ *     stays as it is, also where the scale grows.
  *   So a page begins anew when its first position is written.  A scale is NaN, and the block reads as NaN, from when it is given a value
  *   that is not finite until then.  positions[t] < 0 (padding): nothing is written, q_out of the token is 0.  q, k, v are strided as there,
  *   q_out is contiguous; k_mean may be NULL (no means).  scratch: xdk_kv8_append_scratch_bytes bytes (0 for

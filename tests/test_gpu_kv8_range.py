@@ -96,3 +96,33 @@ def test_selection_of_as_many_pages_as_there_can_be(position):
     assert got[0, 0, :pages].tolist() == list(range(pages))
     for part in got[0, 0, pages:].split(1 << 29):
         assert bool((part == -1).all())
+
+
+@pytest.mark.parametrize("codes", [INT8, E4M3])
+def test_scores_are_near_those_of_exact_means(codes):
+    """A chosen page's score by its exact mean key is below that of no page left out by more than what the rounding of q and of the means
+    is off by: half a step of each, 1/127 of the largest |value| (of the head of q, of the block)."""
+    from cross_dsl_kernels_b200 import kv8
+    page, dim, heads, last, top, g = 16, 64, (4, 2), 60, 12, _gen(36)
+    table, pos = torch.randperm(last + 1, generator=g)[None], torch.arange((last + 1) * page)
+    ours = kv8.PagedKV8Cache.empty(last + 1, page, heads[1], dim, dtype=codes)
+    k = torch.randn(last + 1, 1, heads[1], dim, generator=g) + 0.7 * torch.randn((last + 1) * page, heads[1], dim, generator=g).view(last + 1, page, heads[1], dim)
+    k = k.flatten(0, 1)
+    trig = torch.ones(pos.numel(), 1, device="cuda"), torch.zeros(pos.numel(), 1, device="cuda")  # no rotation
+    kv8.rope_gqa_paged_kv8_append(torch.zeros(pos.numel(), heads[0], dim, device="cuda"), k.cuda(), k.cuda(), *trig, pos.cuda(), table.cuda(),
+                                  torch.zeros_like(pos).cuda(), ours, rope_dim=2, interleaved=False)
+    q = torch.randn(1, heads[0], dim, generator=g)
+    at = pos[-1:].cuda(), table.cuda(), torch.zeros(1, dtype=torch.int64, device="cuda")
+    pages = kv8.select_kv8_pages(q.cuda(), ours, *at, top_pages=top).cpu()
+    means = ours.dequantized()[0].double().cpu()[table[0, :last]].mean(1)  # [pages, heads, dim] of the codes
+    step = ours.k_scale.double().cpu()[table[0, :last]][..., None] * (1.0 if codes == INT8 else 448 / 127)
+    for h in range(heads[1]):
+        x = q[0, h * 2:h * 2 + 2].double()
+        unit = x.abs().amax(-1, keepdim=True) / 127
+        score = (x @ means[:, h].T).amax(0)
+        off = (0.5 * (x.abs()[:, None] * step[None, :, h] + means[None, :, h].abs() * unit[:, None] + 0.5 * step[None, :, h] * unit[:, None])).sum(-1).amax(0)
+        off = off + 2.0 ** -21 * score.abs()  # the FP32 steps of a score
+        chosen = torch.zeros(last, dtype=torch.bool)
+        chosen[pages[0, h, :-1].long()] = True
+        assert chosen.sum() == top - 1 and pages[0, h, -1] == last
+        assert bool(((score + off)[chosen].min() >= (score - off)[~chosen].max()))
