@@ -126,3 +126,20 @@ def test_scores_are_near_those_of_exact_means(codes):
         chosen[pages[0, h, :-1].long()] = True
         assert chosen.sum() == top - 1 and pages[0, h, -1] == last
         assert bool(((score + off)[chosen].min() >= (score - off)[~chosen].max()))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("heads,dim,page,positions", [((8, 2), 128, 16, [0, 15, 300, 5000, -1]), ((6, 2), 64, 7, [1000, 6, 7]), ((5, 1), 256, 32, [63, 0, 700])])
+def test_e4m3_codes_have_no_offset(dtype, heads, dim, page, positions):
+    """Codes of e4m3 enter the products as they are: the limit without what int8 codes are granted for theirs, which is
+    * of a score, 2^-22 of sum |q_d k_d| for each of the 2 dim / 16 truncating products of its chain and for four steps of its scaling,
+    * of a weight, twice that, its rounding to FP16 (2^-11) and FP32 steps of the sums (2^-18),
+    * of the smallest FP16 weights half a step, 2^-39 of the largest, and half a step of the result's type."""
+    from cross_dsl_kernels_b200 import kv8
+    cache, pos, table, seq = _attend_inputs(heads, dim, page, positions, E4M3, seed=37)
+    q = torch.randn(len(positions), heads[0], dim, generator=_gen(37)).to(dtype)
+    exact, info = oracle.attention(q, cache, pos, table, seq), torch.finfo(dtype)
+    weight = 2.0 ** -11 + 2.0 ** -18 + 2 * exact["score"][..., None] * (2 * dim // 16 + 4) * 2.0 ** -22
+    limit = exact["bound"] * weight * 1.01 + exact["least"] * 2.0 ** -39 + exact["result"].abs().clamp(min=info.smallest_normal) * info.eps / 2
+    got = kv8.paged_kv8_decode_attention(q.cuda(), _on_gpu(cache, "HND"), *(t.cuda() for t in (pos, table, seq)))
+    assert bool(((got.double().cpu() - exact["result"]).abs() <= limit).all())
