@@ -345,7 +345,7 @@ struct Kv8Call {
     width = table->size(1);
     return true;
   }
-  bool reads() const { return q->is_contiguous() && hq / hkv <= 8; }
+  bool reads() const { return q->is_contiguous() && hq / hkv <= 8 && tokens <= 65535 && tokens * hkv <= (1 << 26); }
   xdk_peer_out to(const at::Tensor& out) const {
     xdk_peer_out dst = {};
     dst.ptr[0] = out.data_ptr(), dst.world = 1, dst.ld = hq * dim, dst.col0 = 0;
@@ -355,7 +355,7 @@ struct Kv8Call {
 bool scale_of(PyObject* o, int64_t dim, double& scale) {
   if (o != Py_None && !PyFloat_CheckExact(o)) return false;
   scale = o == Py_None ? std::pow(static_cast<double>(dim), -0.5) : PyFloat_AS_DOUBLE(o);
-  return std::isfinite(scale);
+  return std::fabs(scale) <= std::numeric_limits<float>::max();
 }
 
 // (q, k, v, cos, sin, positions, page_table, sequence_ids, <cache: 6>, rope_dim, interleaved, dependent_launch)
@@ -370,6 +370,7 @@ PyObject* kv8_append(PyObject*, PyObject* const* arg, Py_ssize_t n) {
   NEED(k && v && cos && sin);
   for (const at::Tensor* t : {k, v, cos, sin})
     NEED(t->device() == c.q->device() && !t->requires_grad() && t->scalar_type() == (t == k || t == v ? c.q->scalar_type() : at::kFloat));
+  NEED(c.tokens <= (1 << 26) && c.hq <= 65535);
   NEED(k->dim() == 3 && k->size(0) == c.tokens && k->size(1) == c.hkv && k->size(2) == c.dim && v->sizes() == k->sizes());
   for (const at::Tensor* t : {c.q, k, v})
     NEED(t->is_contiguous() || (t->stride(2) == 1 && t->stride(1) == t->size(2) && t->stride(0) >= t->size(1) * t->size(2)));

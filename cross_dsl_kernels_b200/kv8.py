@@ -19,7 +19,6 @@ padding.  These ops have no gradient.
 from __future__ import annotations
 
 import ctypes
-import math
 from dataclasses import dataclass
 
 import torch
@@ -32,6 +31,9 @@ HEAD_DIMS = (64, 128, 256)
 MAX_PAGE_SIZE = 1024
 MAX_GROUP = 8  # query heads that share a KV head
 MAX_SELECT_PAGES = 51200  # pages of a sequence that select_kv8_pages can choose from
+MAX_TOKENS = 65535  # of a call that reads the cache
+MAX_APPEND_TOKENS = 1 << 26  # and tokens * kv_heads of one that reads it
+_LARGEST = 3.4028234663852886e38  # of float32
 _CODES = {torch.int8: _native.XDK_KV8_INT8, torch.float8_e4m3fn: _native.XDK_KV8_E4M3}
 
 
@@ -151,6 +153,8 @@ def rope_gqa_paged_kv8_append(q, k, v, cos, sin, positions, page_table, sequence
     if done is not None:
         return done
     tokens, q_heads = _indices(q, cache, positions, page_table, sequence_ids)
+    _need(tokens <= MAX_APPEND_TOKENS, f"at most {MAX_APPEND_TOKENS} tokens per call")
+    _need(q_heads <= 65535, "q_heads must be at most 65535")
     kv_heads, head_dim = cache.kv_heads, cache.head_dim
     for name, t, want in (("k", k, q.dtype), ("v", v, q.dtype), ("cos", cos, torch.float32), ("sin", sin, torch.float32)):
         _need(t.is_cuda and t.device == q.device, f"{name} must be on the same CUDA device as q")
@@ -197,7 +201,9 @@ def _read(q, cache, positions, page_table, sequence_ids, scale):
     _need(q.is_contiguous(), "q must be contiguous [tokens, q_heads, head_dim]")
     _need(q_heads // cache.kv_heads <= MAX_GROUP, f"q_heads / kv_heads must be at most {MAX_GROUP}")
     scale = float(cache.head_dim) ** -0.5 if scale is None else float(scale)
-    _need(math.isfinite(scale), "scale must be finite")
+    _need(abs(scale) <= _LARGEST, "scale must be finite in float32")
+    _need(tokens <= MAX_TOKENS, f"at most {MAX_TOKENS} tokens per call")
+    _need(tokens * cache.kv_heads <= MAX_APPEND_TOKENS, f"tokens * kv_heads must be at most {MAX_APPEND_TOKENS}")
     return tokens, q_heads, scale
 
 
