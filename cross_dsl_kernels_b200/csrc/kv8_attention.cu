@@ -8,11 +8,12 @@
 // heads of the group as the 8 columns:
 //   * q is scaled by a power of two, so that its largest value is near 2^14, and rounded to FP16 (FP16 and BF16 values pass whole unless
 //     they are 2^-27 of the largest); an FP32 q is the sum of two such numbers, and each product two products.
-//   * the weights are the softmax weights times the block scales of V, w = p * vs = 2^(s + e) * f with vs = 2^e * f, f in [1, 2): the running
-//     maximum of s + e keeps them in range whatever the scales are, that of s alone the sum of the softmax weights.  (One maximum and one exponential
+//   * the weights are the softmax weights times the block scales of V, w = p * vs = 2^(s + log2 vs): the running maximum of s + log2 vs keeps
+//     them in range whatever the scales are, that of s alone the sum of the softmax weights.  (One maximum and one exponential
 //     for both, the sum with vs taken out again, holds for scales within 2^60 of one another; it takes the same time.)  The largest
-//     weight of a head is 2^14 or more, so that what rounds away is below 2^-38 of it; weights are rounded to FP16 (half a step: 2^-11), for FP32
-//     again as the sum of two.
+//     weight of a head is 2^14, which FP16 has, so that what rounds away is below 2^-38 of it; the others are rounded to FP16 (half a step: 2^-11).
+//     For FP32 results the logarithm's rounding would count: the exponent of vs goes with s and its significand is a factor, and a weight is the
+//     sum of two FP16 numbers.
 //   * int8 codes enter as the subnormal halves (code + 128) * 2^-24, which a byte permute makes; the sums begin with -128 times the sum of
 //     the other operand.  FP32 results would see the few 2^-23 of 128 that this rounds away: for them the codes are centred first.
 //   * a tile's sum is added to the accumulators by FP32 FMAs, with rounding; the tensor core truncates.
@@ -59,7 +60,7 @@ template <int D> constexpr int kTileOf = D == 64 ? 64 : 32;  // positions of a t
 inline int tile_of(int64_t dim) { return dim == 64 ? kTileOf<64> : kTileOf<128>; }
 constexpr int kEntry = 2;                    // what the change to another item costs a warp, in tiles
 constexpr int64_t kMaxContextHint = 1LL << 38;
-constexpr float kWeightLog2 = 14.0f;  // the largest weight of a head in FP16 is 2^14 .. 2^15
+constexpr float kWeightLog2 = 14.0f;  // the largest weight of a head in FP16 is 2^14 (SPLIT: up to 2^15)
 
 // A stage: K rows, V rows (16-byte pieces xor-swizzled, so that eight rows of an ldmatrix lie on eight bank groups).
 template <int D>
@@ -300,7 +301,7 @@ kv8_attention_kernel(const __grid_constant__ Kv8Args a, const __grid_constant__ 
   constexpr bool CENTRED = SPLIT;    // FP32 results would see what an offset of the codes cancels
   extern __shared__ __align__(128) unsigned char ring[];
   __shared__ int64_t rows[TP];     // byte offsets of the rows that are fetched
-  __shared__ float4 per_row[TP];   // of a tile's positions: scale of K, 0 (-infinity: dead), significand and exponent of the scale of V
+  __shared__ float4 per_row[TP];   // of a tile's positions: scale of K, 0 (-infinity: dead); of V the significand and the exponent (not SPLIT: the logarithm)
 
   pdl_launch_dependents();
   pdl_wait();  // q and the caches are the preceding kernels' output
@@ -481,8 +482,8 @@ kv8_attention_kernel(const __grid_constant__ Kv8Args a, const __grid_constant__ 
 #pragma unroll
     for (int e = 0; e < 2; ++e) s_zero[e] = -Codec<C>::kOffset * Codec<C>::kUnit * __shfl_sync(0xffffffffu, sum, (2 * quad + e) * 4);
   }
-  // Of heads 2 quad + {0, 1}, in units of log2: the running maxima of s plus the exponent of the scale of V -- what makes the largest weight
-  // 2^kWeightLog2 or more -- and of s, and this thread's share of the sum of the softmax weights 2^(s - s_run).
+  // Of heads 2 quad + {0, 1}, in units of log2: the running maxima of s plus the logarithm (SPLIT: exponent) of the scale of V -- what makes the largest
+  // weight 2^kWeightLog2 or more -- and of s, and this thread's share of the sum of the softmax weights 2^(s - s_run).
   float m_run[2], s_run[2], l_run[2];
   float o[NC][4];  // O^T: dims 16 c + 2 grow (+ 1 in the upper two), the same heads
 #pragma unroll
@@ -502,8 +503,8 @@ kv8_attention_kernel(const __grid_constant__ Kv8Args a, const __grid_constant__ 
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const bool live = !(vs[0][r] < 0.0f);  // NaN is alive
-      float significand = live ? vs[0][r] : 0.0f;
-      const float exponent = split_scale(significand);
+      float significand = live ? vs[0][r] : 0.0f, exponent = split_scale(significand);
+      if constexpr (!SPLIT) exponent += live ? log2_fast(significand) : 0.0f;
       per_row[r * 32 + lane] = make_float4(ks[0][r] * k_lift, live ? 0.0f : -INFINITY, significand, exponent);
 #pragma unroll
       for (int s = 0; s < NST - 1; ++s) ks[s][r] = ks[s + 1][r], vs[s][r] = vs[s + 1][r];
@@ -536,12 +537,13 @@ kv8_attention_kernel(const __grid_constant__ Kv8Args a, const __grid_constant__ 
         }
       }
     // ---- online softmax of the two heads
-    float mx[2] = {m_run[0], m_run[1]}, ms[2] = {s_run[0], s_run[1]};
+    float mx[2] = {m_run[0], m_run[1]}, ms[2] = {s_run[0], s_run[1]}, lv[PB][2];
 #pragma unroll
     for (int pb = 0; pb < PB; ++pb)
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
         const float4 f = per_row[pb * 16 + grow + r * 8];
+        lv[pb][r] = f.w;
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           float& s = sc[pb][2 * r + e];
@@ -570,12 +572,12 @@ kv8_attention_kernel(const __grid_constant__ Kv8Args a, const __grid_constant__ 
     for (int pb = 0; pb < PB; ++pb)
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        const float4 f = per_row[pb * 16 + grow + r * 8];
         float x[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const float s = sc[pb][2 * r + e];
-          x[e] = exp2_fast(s + f.w - from[e]) * f.z, l_run[e] += exp2_fast(s - sum_from[e]);
+          x[e] = exp2_fast(s + lv[pb][r] - from[e]), l_run[e] += exp2_fast(s - sum_from[e]);
+          if constexpr (SPLIT) x[e] *= per_row[pb * 16 + grow + r * 8].z;
         }
         const __half2 hi = __floats2half2_rn(x[0], x[1]);
         wb[0][pb][r] = transpose8x8(*reinterpret_cast<const uint32_t*>(&hi));

@@ -143,3 +143,24 @@ def test_e4m3_codes_have_no_offset(dtype, heads, dim, page, positions):
     limit = exact["bound"] * weight * 1.01 + exact["least"] * 2.0 ** -39 + exact["result"].abs().clamp(min=info.smallest_normal) * info.eps / 2
     got = kv8.paged_kv8_decode_attention(q.cuda(), _on_gpu(cache, "HND"), *(t.cuda() for t in (pos, table, seq)))
     assert bool(((got.double().cpu() - exact["result"]).abs() <= limit).all())
+
+
+@pytest.mark.parametrize("codes", [INT8, E4M3])
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+def test_one_position_that_has_all_the_weight(codes, dtype):
+    """Its weight is rounded to nothing: the result is its value, rounded once to the result's type but for the FP32 steps behind the products."""
+    from cross_dsl_kernels_b200 import kv8
+    cache, pos, table, seq = _attend_inputs((4, 2), 128, 16, [900, 333, 15], codes, seed=38)
+    q = torch.zeros(3, 4, 128)
+    q[..., 0] = 1.0
+    cache["k"].view(torch.uint8)[:, :, :, 0] = 0
+    cache["k_scale"][:] = 40.0
+    exact = torch.zeros(3, 2, 128, dtype=torch.float64)
+    for t, j in enumerate((411, 332, 0)):
+        page, row = int(table[seq[t], j // 16]), j % 16
+        cache["k"][page, row, :, 0] = torch.tensor(64.0).to(codes)  # a score of 64 * 40 / 128 ** 0.5 against zeros
+        exact[t] = cache["v"][page, row].double() * cache["v_scale"][page].double()[:, None]
+    got = kv8.paged_kv8_decode_attention(q.to(dtype).cuda(), _on_gpu(cache, "NHD"), *(t.cuda() for t in (pos, table, seq))).double().cpu()
+    exact = exact.repeat_interleave(2, 1)
+    info = torch.finfo(dtype)
+    assert bool(((got - exact).abs() <= exact.abs().clamp(min=info.smallest_normal) * (info.eps / 2 + 2.0 ** -19)).all())
