@@ -19,9 +19,11 @@
 // us), whose mean its threads sum in slices (by one warp: 50).
 // A lane holds two vectors of eight dims of a row, rotation partners where there are some, and so reads every value and angle once.
 //
-// Bound: a decode batch (3.5 us) by its chain of dependent loads: position, sequence, page, then the block's scale.  4096 tokens: 30 us, where
-// HBM takes 14 (values read once, codes written once; the second launch finds K and V in L2): 2 us for the memset, 6 for the first launch,
-// 5 for the second one's chain of loads, then the rows, bound by the instructions of rotation and exact division.
+// Bound: a decode batch by its chain of dependent loads: position, sequence, page, then the block's scale (3.5 us where no scale grows), and then the
+// rows that a grown scale moves, a few at a time by the block's warp: row 8 of pages of 16 4.1 -> 5.0 us, row 33 of 64 5.0 -> 9.2.  4096 tokens: 30 us,
+// where HBM takes 14 (values read once, codes written once; the second launch finds K and V in L2): 2 us for the memset, 6 for the first launch,
+// 5 for the second one's chain of loads, then the rows, by latency first (57 % of the cycles issue), then by rotation and exact division.
+// A page's tokens are looked for between its first and last one: in random order 65536 tokens of 2 KV heads of 64 take 168 us for 73, 262144 1839 for 305.
 #include <math.h>
 
 #include "kv8.cuh"

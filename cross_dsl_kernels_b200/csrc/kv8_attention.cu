@@ -26,7 +26,7 @@
 // weights, and a second launch adds them in their order.  (Chunks that the hardware hands out as warps finish, by CTAs or by cancelled launches, measured slower: 70 us for 16
 // contexts of 8192, where equal ranges took 61 with the same tiles; a chunk's start costs its warp 6 us without loads.)
 //
-// 32 / 8 heads of 128, us: 16 contexts of 32768 172 (6.2 TB/s), of 8192 57 (4.7), 64 of 1 .. 2048 37, one of 8192 14.  Of short work it is bound by
+// 32 / 8 heads of 128, us: 16 contexts of 32768 175 (6.1 TB/s), of 8192 57 (4.7), 64 of 1 .. 2048 38, one of 8192 14.  Of short work it is bound by
 // its two launches and the chain position -> page table -> rows (8 us), of long work by HBM.
 #include <math.h>
 

@@ -12,7 +12,7 @@
 // loaded during these ones' products: 14.7), and the codes of q stand in registers in the same order of dims.  The scores stay in shared
 // memory as sortable integers; up to three passes over 11, 11 and 10 bits of them find the value of the last one chosen (two, mostly:
 // no other has its first 22 bits), one more writes the pages in order.
-// Bound: 512 pages (7.0 us for one token) by the chain of loads and barriers; 2048 pages, whose means are 35 MB, from HBM (15.6 us) by
+// Bound: 512 pages (7.0 us for one token) by the chain of loads and barriers; 2048 pages, whose means are 35 MB, from HBM (14.8 us) by
 // the latency of their reads: 2.3 us in front of the scores, 10 for them, 3.3 for the choice.
 #include <math.h>
 
