@@ -8,10 +8,11 @@
 // heads of the group as the 8 columns:
 //   * q is scaled by a power of two, so that its largest value is near 2^14, and rounded to FP16 (FP16 and BF16 values pass whole unless
 //     they are 2^-27 of the largest); an FP32 q is the sum of two such numbers, and each product two products.
-//   * the weights are the softmax weights times the block scales of V, w = p * vs = 2^(s + log2 vs): the running maximum of s + log2 vs keeps
-//     them in range whatever the scales are, that of s alone the sum of the softmax weights.  (One maximum and one exponential
-//     for both, the sum with vs taken out again, holds for scales within 2^60 of one another; it takes the same time.)  The largest
-//     weight of a head is 2^14, which FP16 has, so that what rounds away is below 2^-38 of it; the others are rounded to FP16 (half a step: 2^-11).
+//   * the weights are the softmax weights times the block scales of V, w = p * vs = 2^(s - max s + log2 vs): the running maximum of that exponent
+//     keeps them in range whatever the scales are, that of s the sum of the softmax weights.  (One maximum, of s + log2 vs, and one exponential
+//     for both, the sum with vs taken out again, holds for scales within 2^60 of one another; two maxima side by side lose vs in the rounding of a
+//     large s.)  The largest weight of a head is 2^14, which FP16 has, so that what rounds away is below 2^-38 of it; the others are rounded to
+//     FP16 (half a step: 2^-11).
 //     For FP32 results the logarithm's rounding would count: the exponent of vs goes with s and its significand is a factor, and a weight is the
 //     sum of two FP16 numbers.
 //   * int8 codes enter as the subnormal halves (code + 128) * 2^-24, which a byte permute makes; the sums begin with -128 times the sum of
@@ -59,6 +60,9 @@ constexpr int kMaxGroup = 8;                 // heads of a group: columns of a m
 template <int D> constexpr int kTileOf = D == 64 ? 64 : 32;  // positions of a tile: of 8 KB or more
 inline int tile_of(int64_t dim) { return dim == 64 ? kTileOf<64> : kTileOf<128>; }
 constexpr int kEntry = 2;                    // what the change to another item costs a warp, in tiles
+// A maximum of nothing: finite, so that differences of two are numbers, and a score of -infinity is infinitely far below it.
+constexpr float kNone = -3.0e38f;
+constexpr float kLeastWeight = -256.0f;      // log2 of weights below which no result comes
 constexpr int64_t kMaxContextHint = 1LL << 38;
 constexpr float kWeightLog2 = 14.0f;  // the largest weight of a head in FP16 is 2^14 (SPLIT: up to 2^15)
 
@@ -482,12 +486,13 @@ kv8_attention_kernel(const __grid_constant__ Kv8Args a, const __grid_constant__ 
 #pragma unroll
     for (int e = 0; e < 2; ++e) s_zero[e] = -Codec<C>::kOffset * Codec<C>::kUnit * __shfl_sync(0xffffffffu, sum, (2 * quad + e) * 4);
   }
-  // Of heads 2 quad + {0, 1}, in units of log2: the running maxima of s plus the logarithm (SPLIT: exponent) of the scale of V -- what makes the largest
-  // weight 2^kWeightLog2 or more -- and of s, and this thread's share of the sum of the softmax weights 2^(s - s_run).
-  float m_run[2], s_run[2], l_run[2];
+  // Of heads 2 quad + {0, 1}, in units of log2: the running maximum of s; that of (s - s_run) plus the logarithm (SPLIT: exponent) of the scale of
+  // V, which makes the largest weight 2^kWeightLog2 or more and is of ordinary size however large the scores are (at least kLeastWeight, so that
+  // it keeps its bits); and this thread's share of the sum of the softmax weights 2^(s - s_run).
+  float s_run[2], w_run[2], l_run[2];
   float o[NC][4];  // O^T: dims 16 c + 2 grow (+ 1 in the upper two), the same heads
 #pragma unroll
-  for (int e = 0; e < 2; ++e) m_run[e] = s_run[e] = -INFINITY, l_run[e] = 0.0f;
+  for (int e = 0; e < 2; ++e) s_run[e] = kNone, w_run[e] = kLeastWeight, l_run[e] = 0.0f;
 #pragma unroll
   for (int c = 0; c < NC; ++c)
 #pragma unroll
@@ -537,7 +542,7 @@ kv8_attention_kernel(const __grid_constant__ Kv8Args a, const __grid_constant__ 
         }
       }
     // ---- online softmax of the two heads
-    float mx[2] = {m_run[0], m_run[1]}, ms[2] = {s_run[0], s_run[1]}, lv[PB][2];
+    float ms[2] = {s_run[0], s_run[1]}, lv[PB][2];
 #pragma unroll
     for (int pb = 0; pb < PB; ++pb)
 #pragma unroll
@@ -548,23 +553,39 @@ kv8_attention_kernel(const __grid_constant__ Kv8Args a, const __grid_constant__ 
         for (int e = 0; e < 2; ++e) {
           float& s = sc[pb][2 * r + e];
           s = fmaf(s, f.x * unit[e], f.y);
-          ms[e] = fmaxf(ms[e], s), mx[e] = fmaxf(mx[e], s + f.w);
+          ms[e] = fmaxf(ms[e], s);
         }
       }
-    auto rebase = [&](float& run, float most) {  // to a maximum of all lanes; returns what the sums so far take
+    auto over_lanes = [&](float most) {
 #pragma unroll
       for (int sh = 4; sh < 32; sh <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, sh));
-      const float by = most == -INFINITY ? 1.0f : exp2_fast(run - most);  // nothing yet
-      run = most;
-      return by;
+      return most;
     };
-    float corr[2], from[2], sum_from[2];
+    float corr[2], mw[2];
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      corr[e] = rebase(m_run[e], mx[e]);
-      l_run[e] *= rebase(s_run[e], ms[e]);
-      from[e] = m_run[e] == -INFINITY ? 0.0f : m_run[e] - kWeightLog2;
-      sum_from[e] = s_run[e] == -INFINITY ? 0.0f : s_run[e];
+      ms[e] = over_lanes(ms[e]);
+      const float back = s_run[e] - ms[e];
+      s_run[e] = ms[e];
+      l_run[e] *= exp2_fast(back);
+      corr[e] = back + w_run[e];
+      mw[e] = fmaxf(corr[e], kLeastWeight);
+    }
+#pragma unroll
+    for (int pb = 0; pb < PB; ++pb)
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float& s = sc[pb][2 * r + e];
+          s -= s_run[e];
+          l_run[e] += exp2_fast(s);
+          mw[e] = fmaxf(mw[e], s + lv[pb][r]);
+        }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      w_run[e] = over_lanes(mw[e]);
+      corr[e] = exp2_fast(corr[e] - w_run[e]);
     }
     uint32_t wb[NQ][PB][2];  // w^T as B fragments: positions 16 pb + 2 quad + {0,1} (+ 8 in [1]), head grow
     float t_zero[2] = {0.0f, 0.0f};  // as s_zero: kOffset * the tile's weights
@@ -575,8 +596,7 @@ kv8_attention_kernel(const __grid_constant__ Kv8Args a, const __grid_constant__ 
         float x[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const float s = sc[pb][2 * r + e];
-          x[e] = exp2_fast(s + lv[pb][r] - from[e]), l_run[e] += exp2_fast(s - sum_from[e]);
+          x[e] = exp2_fast(sc[pb][2 * r + e] + lv[pb][r] - (w_run[e] - kWeightLog2));
           if constexpr (SPLIT) x[e] *= per_row[pb * 16 + grow + r * 8].z;
         }
         const __half2 hi = __floats2half2_rn(x[0], x[1]);
@@ -645,9 +665,9 @@ kv8_attention_kernel(const __grid_constant__ Kv8Args a, const __grid_constant__ 
     for (int sh = 4; sh < 32; sh <<= 1) l_run[e] += __shfl_xor_sync(0xffffffffu, l_run[e], sh);
     const int head = quad * 2 + e;
     if (head >= G) continue;
-    // o / l times 2^(m_run - kWeightLog2 - s_run), in two halves, which keeps what is on the way in range
+    // o / l times 2^(w_run - kWeightLog2), in two halves, which keeps what is on the way in range
     const float each = l_run[e] == 0.0f ? 0.0f : 1.0f / l_run[e] * kValueUnit;
-    const float half = m_run[e] == -INFINITY ? 0.0f : exp2_fast(0.5f * (m_run[e] - kWeightLog2 - s_run[e]));
+    const float half = exp2_fast(0.5f * (w_run[e] - kWeightLog2));
     auto value = [&](int c, int i) { return o[c][e + 2 * i] * half * each * half; };
     if (whole) {
       store_dims<SPLIT>(out, token, static_cast<int64_t>(kvh * G + head) * D + 2 * grow, a.dtype, a.paired, value, std::integral_constant<int, NC>());
@@ -677,10 +697,10 @@ template <int N> __device__ __forceinline__ void add_parts(Part& sum, const Part
   float m = sum.m;
 #pragma unroll
   for (int i = 0; i < N; ++i) m = fmaxf(m, p[i].m);
-  const float from = m == -INFINITY ? 0.0f : m, had = exp2_fast(0.5f * (sum.m - from));
+  const float had = exp2_fast(0.5f * (sum.m - m));
   float half[N], l = sum.l * had * had;
 #pragma unroll
-  for (int i = 0; i < N; ++i) half[i] = exp2_fast(0.5f * (p[i].m - from)), l += p[i].l * half[i] * half[i];
+  for (int i = 0; i < N; ++i) half[i] = exp2_fast(0.5f * (p[i].m - m)), l += p[i].l * half[i] * half[i];
   const float per = l == 0.0f ? 0.0f : 1.0f / l;
   float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   auto add = [&](const Part& part, float h) {
@@ -713,7 +733,7 @@ kv8_attention_merge_kernel(const __grid_constant__ Kv8Args a, const __grid_const
   const int item = a.by_warp ? share.x : blockIdx.x, begins = a.by_warp ? blockIdx.x : share.x;
   const bool some = at < all;
   const int head = some ? at / dim : 0;
-  const Part none = {make_float4(0.0f, 0.0f, 0.0f, 0.0f), -INFINITY, 0.0f};
+  const Part none = {make_float4(0.0f, 0.0f, 0.0f, 0.0f), kNone, 0.0f};
   Part sum = none, p[N];
 #pragma unroll 1
   for (int first = group; first < share.y; first += kGroups * N) {

@@ -164,3 +164,34 @@ def test_one_position_that_has_all_the_weight(codes, dtype):
     exact = exact.repeat_interleave(2, 1)
     info = torch.finfo(dtype)
     assert bool(((got - exact).abs() <= exact.abs().clamp(min=info.smallest_normal) * (info.eps / 2 + 2.0 ** -19)).all())
+
+
+@pytest.mark.parametrize("codes", [INT8, E4M3])
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("k_scale", [3e3, 1e5, 1e7, 1e12, 1e30])
+def test_scores_of_any_size(codes, dtype, k_scale):
+    """Scores between which one step of FP32 is more than the logarithms of V's scales: a position that has all the weight gives its value; where
+    its scale of V is 0, nothing."""
+    from cross_dsl_kernels_b200 import kv8
+    cache, pos, table, seq = _attend_inputs((4, 2), 128, 16, [900, 333, 15], codes, seed=39)
+    q = torch.zeros(3, 4, 128)
+    q[..., 0] = 1.0
+    cache["k"].view(torch.uint8)[:, :, :, 0] = 0
+    cache["k_scale"][:] = k_scale
+    exact = torch.zeros(3, 2, 128, dtype=torch.float64)
+    for t, j in enumerate((411, 332, 0)):
+        page, row = int(table[seq[t], j // 16]), j % 16
+        for at, code in ((page, 64.0), (int(table[seq[t], 0]), -32.0)):  # the largest score, and one far below the rest's zeros
+            cache["k"][at, row if code > 0 else 3, :, 0] = torch.tensor(code).to(codes)
+        exact[t] = cache["v"][page, row].double() * cache["v_scale"][page].double()[:, None]
+    info = torch.finfo(dtype)
+
+    def read(kept):
+        got = kv8.paged_kv8_decode_attention(q.to(dtype).cuda(), _on_gpu(cache, "NHD"), *(t.cuda() for t in (pos, table, seq))).double().cpu()
+        want = (exact * kept).repeat_interleave(2, 1)
+        assert bool(((got - want).abs() <= want.abs().clamp(min=info.smallest_normal) * (info.eps / 2 + 2.0 ** -19)).all())
+
+    read(1.0)
+    for t, j in enumerate((411, 332, 0)):
+        cache["v_scale"][table[seq[t], j // 16]] = 0
+    read(0.0)
