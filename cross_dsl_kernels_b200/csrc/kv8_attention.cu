@@ -10,8 +10,8 @@
 //     they are 2^-27 of the largest); an FP32 q is the sum of two such numbers, and each product two products.
 //   * the weights are the softmax weights times the block scales of V, w = p * vs = 2^(s - max s + log2 vs): the running maximum of that exponent
 //     keeps them in range whatever the scales are, that of s the sum of the softmax weights.  (One maximum, of s + log2 vs, and one exponential
-//     for both, the sum with vs taken out again, holds for scales within 2^60 of one another; two maxima side by side lose vs in the rounding of a
-//     large s.)  The largest weight of a head is 2^14, which FP16 has, so that what rounds away is below 2^-38 of it; the others are rounded to
+//     for both, the sum with vs taken out again, holds for scales within 2^60 of one another, and takes 2 - 4 % less; two maxima side by side lose vs
+//     in the rounding of a large s.)  The largest weight of a head is 2^14, which FP16 has, so that what rounds away is below 2^-38 of it; the others are rounded to
 //     FP16 (half a step: 2^-11).
 //     For FP32 results the logarithm's rounding would count: the exponent of vs goes with s and its significand is a factor, and a weight is the
 //     sum of two FP16 numbers.
@@ -27,7 +27,7 @@
 // weights, and a second launch adds them in their order.  (Chunks that the hardware hands out as warps finish, by CTAs or by cancelled launches, measured slower: 70 us for 16
 // contexts of 8192, where equal ranges took 61 with the same tiles; a chunk's start costs its warp 6 us without loads.)
 //
-// 32 / 8 heads of 128, us: 16 contexts of 32768 175 (6.1 TB/s), of 8192 57 (4.7), 64 of 1 .. 2048 38, one of 8192 14.  Of short work it is bound by
+// 32 / 8 heads of 128, us: 16 contexts of 32768 179 (6.0 TB/s), of 8192 57 (4.7), 64 of 1 .. 2048 39, one of 8192 14.  Of short work it is bound by
 // its two launches and the chain position -> page table -> rows (8 us), of long work by HBM.
 #include <math.h>
 
@@ -580,7 +580,8 @@ kv8_attention_kernel(const __grid_constant__ Kv8Args a, const __grid_constant__ 
           float& s = sc[pb][2 * r + e];
           s -= s_run[e];
           l_run[e] += exp2_fast(s);
-          mw[e] = fmaxf(mw[e], s + lv[pb][r]);
+          s += lv[pb][r];
+          mw[e] = fmaxf(mw[e], s);
         }
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
@@ -596,7 +597,7 @@ kv8_attention_kernel(const __grid_constant__ Kv8Args a, const __grid_constant__ 
         float x[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          x[e] = exp2_fast(sc[pb][2 * r + e] + lv[pb][r] - (w_run[e] - kWeightLog2));
+          x[e] = exp2_fast(sc[pb][2 * r + e] - (w_run[e] - kWeightLog2));
           if constexpr (SPLIT) x[e] *= per_row[pb * 16 + grow + r * 8].z;
         }
         const __half2 hi = __floats2half2_rn(x[0], x[1]);
