@@ -8,13 +8,13 @@
 // heads of the group as the 8 columns:
 //   * q is scaled by a power of two, so that its largest value is near 2^14, and rounded to FP16 (FP16 and BF16 values pass whole unless
 //     they are 2^-27 of the largest); an FP32 q is the sum of two such numbers, and each product two products.
-//   * the weights are the softmax weights times the block scales of V, w = p * vs = 2^(s - max s + log2 vs): the running maximum of that exponent
-//     keeps them in range whatever the scales are, that of s the sum of the softmax weights.  (One maximum, of s + log2 vs, and one exponential
-//     for both, the sum with vs taken out again, holds for scales within 2^60 of one another, and takes 2 - 4 % less; two maxima side by side lose vs
-//     in the rounding of a large s.)  The largest weight of a head is 2^14, which FP16 has, so that what rounds away is below 2^-38 of it; the others are rounded to
-//     FP16 (half a step: 2^-11).
-//     For FP32 results the logarithm's rounding would count: the exponent of vs goes with s and its significand is a factor, and a weight is the
-//     sum of two FP16 numbers.
+//   * the weights are the softmax weights times the block scales of V, w = p * vs = 2^(s + log2 vs): one running maximum, of the whole exponent,
+//     and one exponential; the softmax sum takes vs out again.  That holds while the scales of V are within 2^30 of the first tile's.  From a tile
+//     on that has one farther away, or 0, the sum has a maximum and an exponential of its own, and the weights are 2^(s - max s + log2 vs), which
+//     large scores do not take the scale from (this for every tile: 2 - 3 % more time).  The largest weight of a head is 2^14, which FP16 has, so that
+//     what rounds away is below 2^-38 of it; the others are rounded to FP16 (half a step: 2^-11).
+//     For FP32 results a weight is the sum of two FP16 numbers, and the logarithm of a far vs would be off by too much: its exponent goes with s, its
+//     significand is a factor.
 //   * int8 codes enter as the subnormal halves (code + 128) * 2^-24, which a byte permute makes; the sums begin with -128 times the sum of
 //     the other operand.  FP32 results would see the few 2^-23 of 128 that this rounds away: for them the codes are centred first.
 //   * a tile's sum is added to the accumulators by FP32 FMAs, with rounding; the tensor core truncates.
@@ -27,7 +27,7 @@
 // weights, and a second launch adds them in their order.  (Chunks that the hardware hands out as warps finish, by CTAs or by cancelled launches, measured slower: 70 us for 16
 // contexts of 8192, where equal ranges took 61 with the same tiles; a chunk's start costs its warp 6 us without loads.)
 //
-// 32 / 8 heads of 128, us: 16 contexts of 32768 179 (6.0 TB/s), of 8192 57 (4.7), 64 of 1 .. 2048 39, one of 8192 14.  Of short work it is bound by
+// 32 / 8 heads of 128, us: 16 contexts of 32768 176 (6.1 TB/s), of 8192 57 (4.7), 64 of 1 .. 2048 38, one of 8192 14.  Of short work it is bound by
 // its two launches and the chain position -> page table -> rows (8 us), of long work by HBM.
 #include <math.h>
 
@@ -60,10 +60,11 @@ constexpr int kMaxGroup = 8;                 // heads of a group: columns of a m
 template <int D> constexpr int kTileOf = D == 64 ? 64 : 32;  // positions of a tile: of 8 KB or more
 inline int tile_of(int64_t dim) { return dim == 64 ? kTileOf<64> : kTileOf<128>; }
 constexpr int kEntry = 2;                    // what the change to another item costs a warp, in tiles
+constexpr int64_t kMaxContextHint = 1LL << 38;
 // A maximum of nothing: finite, so that differences of two are numbers, and a score of -infinity is infinitely far below it.
 constexpr float kNone = -3.0e38f;
-constexpr float kLeastWeight = -256.0f;      // log2 of weights below which no result comes
-constexpr int64_t kMaxContextHint = 1LL << 38;
+constexpr float kNear = 1073741824.0f;  // 2^30: scales of V within that of their unit are near it
+constexpr float kLeastWeight = -256.0f; // log2 of weights below which no result comes; no maximum of theirs is lower, which keeps its bits
 constexpr float kWeightLog2 = 14.0f;  // the largest weight of a head in FP16 is 2^14 (SPLIT: up to 2^15)
 
 // A stage: K rows, V rows (16-byte pieces xor-swizzled, so that eight rows of an ldmatrix lie on eight bank groups).
@@ -158,6 +159,12 @@ __device__ __forceinline__ void store_dims(const PeerOut& out, int64_t row, int6
       }
     }
   }
+}
+// What the exponents of the weights are taken from for a maximum of `most`: kWeightLog2 below it, as far as a large one shows that; at most 15,
+// so that no weight passes FP16.
+__device__ __forceinline__ float weights_from(float most) {
+  const float from = most - kWeightLog2;
+  return most - from <= 15.0f ? from : most;
 }
 // The e of a scale that is not below 0 as 2^e * f, f in [1, 2), which takes its place; 0: 2^-infinity times 0, what is not finite: 2^0 times that.
 __device__ __forceinline__ float split_scale(float& scale) {
@@ -305,7 +312,8 @@ kv8_attention_kernel(const __grid_constant__ Kv8Args a, const __grid_constant__ 
   constexpr bool CENTRED = SPLIT;    // FP32 results would see what an offset of the codes cancels
   extern __shared__ __align__(128) unsigned char ring[];
   __shared__ int64_t rows[TP];     // byte offsets of the rows that are fetched
-  __shared__ float4 per_row[TP];   // of a tile's positions: scale of K, 0 (-infinity: dead); of V the significand and the exponent (not SPLIT: the logarithm)
+  __shared__ float4 per_row[TP];   // of a tile's positions: scale of K; of V as `far` takes it
+  __shared__ float s_max[kMaxGroup];  // see `far`
 
   pdl_launch_dependents();
   pdl_wait();  // q and the caches are the preceding kernels' output
@@ -486,13 +494,15 @@ kv8_attention_kernel(const __grid_constant__ Kv8Args a, const __grid_constant__ 
 #pragma unroll
     for (int e = 0; e < 2; ++e) s_zero[e] = -Codec<C>::kOffset * Codec<C>::kUnit * __shfl_sync(0xffffffffu, sum, (2 * quad + e) * 4);
   }
-  // Of heads 2 quad + {0, 1}, in units of log2: the running maximum of s; that of (s - s_run) plus the logarithm (SPLIT: exponent) of the scale of
-  // V, which makes the largest weight 2^kWeightLog2 or more and is of ordinary size however large the scores are (at least kLeastWeight, so that
-  // it keeps its bits); and this thread's share of the sum of the softmax weights 2^(s - s_run).
-  float s_run[2], w_run[2], l_run[2];
+  // Scales of V are taken in units of v_unit, the power of two of the largest in the first tile, as long as all of them are near it.  Of heads
+  // 2 quad + {0, 1}: w_run, the running maximum of s + log2(vs / v_unit), in units of log2, which makes the largest weight 2^kWeightLog2, and this
+  // thread's share of the sum of the softmax weights, l_run: the weights with vs / v_unit taken out again.
+  // far (v_unit is 0): from the first tile on that has a scale that is not near it, 0 among them, the sum is that of 2^(s - s_max), s_max the
+  // running maximum of s, and w_run that of (s - s_max) + log2 vs (SPLIT: the exponent of vs, whose significand is a factor then).
+  float w_run[2], l_run[2], v_unit = 1.0f;
   float o[NC][4];  // O^T: dims 16 c + 2 grow (+ 1 in the upper two), the same heads
 #pragma unroll
-  for (int e = 0; e < 2; ++e) s_run[e] = kNone, w_run[e] = kLeastWeight, l_run[e] = 0.0f;
+  for (int e = 0; e < 2; ++e) w_run[e] = kNone, l_run[e] = 0.0f;
 #pragma unroll
   for (int c = 0; c < NC; ++c)
 #pragma unroll
@@ -505,12 +515,43 @@ kv8_attention_kernel(const __grid_constant__ Kv8Args a, const __grid_constant__ 
 
   for (int u = first; u < end; ++u) {
     fetch_next(stage == 0 ? NST - 1 : stage - 1, ks[NST - 1], vs[NST - 1]);
+    if (u == first) {
+      float most = vs[0][0];
+#pragma unroll
+      for (int r = 1; r < R; ++r) most = fmaxf(most, vs[0][r]);
+#pragma unroll
+      for (int sh = 16; sh > 0; sh >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, sh));
+      if (most > 1e-37f && most < 8e37f) v_unit = __uint_as_float(__float_as_uint(most) & 0x7f800000u);  // 2^-123 .. 2^125
+    }
+    const float to_unit = __uint_as_float(0x7f000000u - __float_as_uint(v_unit));  // one over it
+    bool leaves = false;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {  // not NaN, which shows either way
+      const float rel = vs[0][r] * to_unit;
+      leaves = leaves || (rel >= 0.0f && !(rel >= 1.0f / kNear && rel <= kNear));
+    }
+    if (v_unit != 0.0f && __any_sync(0xffffffffu, leaves)) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {  // l_run is a sum of 2^(s - weights_from(w_run)) so far
+        const bool none = w_run[e] == kNone;
+        if (grow == 0) s_max[2 * quad + e] = none ? kNone : weights_from(w_run[e]);
+        w_run[e] = none ? kLeastWeight : static_cast<float>(static_cast<int>(__float_as_uint(v_unit) >> 23) - 127) + kWeightLog2;
+      }
+      v_unit = 0.0f;
+    }
+    const bool far = v_unit == 0.0f;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const bool live = !(vs[0][r] < 0.0f);  // NaN is alive
-      float significand = live ? vs[0][r] : 0.0f, exponent = split_scale(significand);
-      if constexpr (!SPLIT) exponent += live ? log2_fast(significand) : 0.0f;
-      per_row[r * 32 + lane] = make_float4(ks[0][r] * k_lift, live ? 0.0f : -INFINITY, significand, exponent);
+      float4& of = per_row[r * 32 + lane];
+      if (!far) {  // log2 (-infinity: dead) and one over it
+        const float in_exponent = log2_fast(vs[0][r] * to_unit);
+        of = make_float4(ks[0][r] * k_lift, live ? in_exponent : -INFINITY, live ? exp2_fast(-in_exponent) : 0.0f, 0.0f);
+      } else {  // 0 (-infinity: dead), significand, and logarithm (SPLIT: exponent)
+        float significand = live ? vs[0][r] : 0.0f, exponent = split_scale(significand);
+        if constexpr (!SPLIT) exponent += live ? log2_fast(significand) : 0.0f;
+        of = make_float4(ks[0][r] * k_lift, live ? 0.0f : -INFINITY, significand, exponent);
+      }
 #pragma unroll
       for (int s = 0; s < NST - 1; ++s) ks[s][r] = ks[s + 1][r], vs[s][r] = vs[s + 1][r];
     }
@@ -542,72 +583,105 @@ kv8_attention_kernel(const __grid_constant__ Kv8Args a, const __grid_constant__ 
         }
       }
     // ---- online softmax of the two heads
-    float ms[2] = {s_run[0], s_run[1]}, lv[PB][2];
-#pragma unroll
-    for (int pb = 0; pb < PB; ++pb)
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const float4 f = per_row[pb * 16 + grow + r * 8];
-        lv[pb][r] = f.w;
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float& s = sc[pb][2 * r + e];
-          s = fmaf(s, f.x * unit[e], f.y);
-          ms[e] = fmaxf(ms[e], s);
-        }
-      }
+    uint32_t wb[NQ][PB][2];  // w^T as B fragments: positions 16 pb + 2 quad + {0,1} (+ 8 in [1]), head grow
+    float corr[2], t_zero[2] = {0.0f, 0.0f};  // what o takes for the new maximum; as s_zero: kOffset * the tile's weights
     auto over_lanes = [&](float most) {
 #pragma unroll
       for (int sh = 4; sh < 32; sh <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, sh));
       return most;
     };
-    float corr[2], mw[2];
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      ms[e] = over_lanes(ms[e]);
-      const float back = s_run[e] - ms[e];
-      s_run[e] = ms[e];
-      l_run[e] *= exp2_fast(back);
-      corr[e] = back + w_run[e];
-      mw[e] = fmaxf(corr[e], kLeastWeight);
-    }
-#pragma unroll
-    for (int pb = 0; pb < PB; ++pb)
-#pragma unroll
-      for (int r = 0; r < 2; ++r)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float& s = sc[pb][2 * r + e];
-          s -= s_run[e];
-          l_run[e] += exp2_fast(s);
-          s += lv[pb][r];
-          mw[e] = fmaxf(mw[e], s);
-        }
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      w_run[e] = over_lanes(mw[e]);
-      corr[e] = exp2_fast(corr[e] - w_run[e]);
-    }
-    uint32_t wb[NQ][PB][2];  // w^T as B fragments: positions 16 pb + 2 quad + {0,1} (+ 8 in [1]), head grow
-    float t_zero[2] = {0.0f, 0.0f};  // as s_zero: kOffset * the tile's weights
-#pragma unroll
-    for (int pb = 0; pb < PB; ++pb)
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        float x[2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          x[e] = exp2_fast(sc[pb][2 * r + e] - (w_run[e] - kWeightLog2));
-          if constexpr (SPLIT) x[e] *= per_row[pb * 16 + grow + r * 8].z;
-        }
-        const __half2 hi = __floats2half2_rn(x[0], x[1]);
-        wb[0][pb][r] = transpose8x8(*reinterpret_cast<const uint32_t*>(&hi));
-        if constexpr (SPLIT || Codec<C>::kOffset != 0.0f) {
-          const float2 h = __half22float2(hi);
-          if constexpr (SPLIT) wb[NQ - 1][pb][r] = transpose8x8(Mma16816<__half>::pack(x[0] - h.x, x[1] - h.y));
-          else t_zero[0] += h.x, t_zero[1] += h.y;
-        }
+    auto put_weights = [&](int pb, int r, float x0, float x1) {
+      const __half2 hi = __floats2half2_rn(x0, x1);
+      wb[0][pb][r] = transpose8x8(*reinterpret_cast<const uint32_t*>(&hi));
+      if constexpr (SPLIT || Codec<C>::kOffset != 0.0f) {
+        const float2 h = __half22float2(hi);
+        if constexpr (SPLIT) wb[NQ - 1][pb][r] = transpose8x8(Mma16816<__half>::pack(x0 - h.x, x1 - h.y));
+        else t_zero[0] += h.x, t_zero[1] += h.y;
       }
+    };
+    if (!far) {
+      float mw[2] = {w_run[0], w_run[1]}, take_out[PB][2];
+#pragma unroll
+      for (int pb = 0; pb < PB; ++pb)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const float4 f = per_row[pb * 16 + grow + r * 8];
+          take_out[pb][r] = f.z;
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float& s = sc[pb][2 * r + e];
+            s = fmaf(s, f.x * unit[e], f.y);
+            mw[e] = fmaxf(mw[e], s);
+          }
+        }
+      float from[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        mw[e] = over_lanes(mw[e]);
+        from[e] = weights_from(mw[e]);
+        corr[e] = exp2_fast(weights_from(w_run[e]) - from[e]);
+        w_run[e] = mw[e];
+        l_run[e] *= corr[e];
+      }
+#pragma unroll
+      for (int pb = 0; pb < PB; ++pb)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const float x0 = exp2_fast(sc[pb][2 * r] - from[0]), x1 = exp2_fast(sc[pb][2 * r + 1] - from[1]);
+          l_run[0] = fmaf(x0, take_out[pb][r], l_run[0]), l_run[1] = fmaf(x1, take_out[pb][r], l_run[1]);
+          put_weights(pb, r, x0, x1);
+        }
+    } else {
+      float ms[2] = {s_max[2 * quad], s_max[2 * quad + 1]}, mw[2];
+      const float before[2] = {ms[0], ms[1]};
+#pragma unroll
+      for (int pb = 0; pb < PB; ++pb)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const float4 f = per_row[pb * 16 + grow + r * 8];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float& s = sc[pb][2 * r + e];
+            s = fmaf(s, f.x * unit[e], f.y);
+            ms[e] = fmaxf(ms[e], s);
+          }
+        }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        ms[e] = over_lanes(ms[e]);
+        if (grow == 0) s_max[2 * quad + e] = ms[e];  // all lanes have read it: the shuffles stand between
+        const float back = before[e] - ms[e];
+        l_run[e] *= exp2_fast(back);
+        corr[e] = back + w_run[e];
+        mw[e] = fmaxf(corr[e], kLeastWeight);
+      }
+#pragma unroll
+      for (int pb = 0; pb < PB; ++pb)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const float in_exponent = per_row[pb * 16 + grow + r * 8].w;
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float& s = sc[pb][2 * r + e];
+            s -= ms[e];
+            l_run[e] += exp2_fast(s);
+            s += in_exponent;
+            mw[e] = fmaxf(mw[e], s);
+          }
+        }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        w_run[e] = over_lanes(mw[e]);
+        corr[e] = exp2_fast(corr[e] - w_run[e]);
+      }
+#pragma unroll
+      for (int pb = 0; pb < PB; ++pb)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const float factor = SPLIT ? per_row[pb * 16 + grow + r * 8].z : 1.0f;
+          put_weights(pb, r, exp2_fast(sc[pb][2 * r] - (w_run[0] - kWeightLog2)) * factor, exp2_fast(sc[pb][2 * r + 1] - (w_run[1] - kWeightLog2)) * factor);
+        }
+    }
     if constexpr (!CENTRED && Codec<C>::kOffset != 0.0f) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
@@ -666,10 +740,15 @@ kv8_attention_kernel(const __grid_constant__ Kv8Args a, const __grid_constant__ 
     for (int sh = 4; sh < 32; sh <<= 1) l_run[e] += __shfl_xor_sync(0xffffffffu, l_run[e], sh);
     const int head = quad * 2 + e;
     if (head >= G) continue;
-    // o / l times 2^(w_run - kWeightLog2), in two halves, which keeps what is on the way in range
+    // o / l, then the unit of V; far: 2^(w_run - kWeightLog2), in two halves.  In turn, which keeps what is on the way in range.
     const float each = l_run[e] == 0.0f ? 0.0f : 1.0f / l_run[e] * kValueUnit;
-    const float half = exp2_fast(0.5f * (w_run[e] - kWeightLog2));
-    auto value = [&](int c, int i) { return o[c][e + 2 * i] * half * each * half; };
+    float value_unit = v_unit, m = weights_from(w_run[e]);
+    if (v_unit == 0.0f) {
+      value_unit = exp2_fast(0.5f * (w_run[e] - kWeightLog2)), m = s_max[head];
+#pragma unroll
+      for (int c = 0; c < NC; ++c) o[c][e] *= value_unit, o[c][e + 2] *= value_unit;
+    }
+    auto value = [&](int c, int i) { return o[c][e + 2 * i] * each * value_unit; };
     if (whole) {
       store_dims<SPLIT>(out, token, static_cast<int64_t>(kvh * G + head) * D + 2 * grow, a.dtype, a.paired, value, std::integral_constant<int, NC>());
     } else {
@@ -677,7 +756,7 @@ kv8_attention_kernel(const __grid_constant__ Kv8Args a, const __grid_constant__ 
 #pragma unroll
       for (int c = 0; c < NC; ++c) *reinterpret_cast<float2*>(to + c * 16) = make_float2(value(c, 0), value(c, 1));
       if (grow == 0) {
-        part.m[slot * kMaxGroup + head] = s_run[e];
+        part.m[slot * kMaxGroup + head] = m;
         part.l[slot * kMaxGroup + head] = l_run[e];
       }
     }
